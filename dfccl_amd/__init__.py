@@ -9,3 +9,4 @@ from .api import (  # noqa: F401
     ncclSum, ncclProd, ncclMax, ncclMin, ncclAvg, ncclInt8, ncclUint8, ncclInt32, ncclUint32, ncclInt64, ncclUint64,
     ncclFloat16, ncclFloat32, ncclFloat64, ncclBfloat16,
 )
+from .indexed import PageCache, embedding_grad, embedding_grad_workspace, embedding_lookup  # noqa: F401

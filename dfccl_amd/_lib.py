@@ -29,8 +29,17 @@ class CollGeometry(ctypes.Structure):
                 ("fifoSlots", ctypes.c_int), ("protocol", ctypes.c_int)]
 
 
+class PageCacheStruct(ctypes.Structure):
+    _fields_ = [("structBytes", ctypes.c_uint64), ("pools", ctypes.POINTER(ctypes.c_void_p)),
+                ("pageBytes", ctypes.c_size_t), ("npools", ctypes.c_int), ("pages", ctypes.c_int),
+                ("pageTokens", ctypes.c_int), ("sequences", ctypes.c_int), ("pagesPerSequence", ctypes.c_int),
+                ("refcounts", ctypes.c_void_p), ("tables", ctypes.c_void_p), ("lengths", ctypes.c_void_p),
+                ("report", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspaceBytes", ctypes.c_size_t)]
+
+
 # every symbol include/ofccl.h declares: name -> (restype, argtypes)
 _vp, _sz, _int = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int
+_i64, _dbl, _cache = ctypes.c_int64, ctypes.c_double, ctypes.POINTER(PageCacheStruct)
 SIGNATURES = {
     "ncclGetUniqueId": (_int, [ctypes.POINTER(UniqueId)]),
     "ncclCommInitRank": (_int, [ctypes.POINTER(_vp), _int, UniqueId, _int]),
@@ -57,6 +66,16 @@ SIGNATURES = {
     "ofcclRunReduceScatter": (_int, [_vp, _vp, _int, CALLBACK, _vp, _vp]),
     "ofcclRunAllGather": (_int, [_vp, _vp, _int, CALLBACK, _vp, _vp]),
     "dfcclReduceCopy": (_int, [ctypes.POINTER(_vp), _int, _vp, _sz, _int, _int, _sz, _vp]),
+    "dfcclEmbeddingLookup": (_int, [_vp, _int, _sz, _sz, _i64, _vp, _int, _sz, _sz, _dbl, _vp, _int, _sz, _vp]),
+    "dfcclEmbeddingGradWorkspace": (_int, [_int, ctypes.POINTER(_sz), _sz, _sz, ctypes.POINTER(_sz)]),
+    "dfcclEmbeddingGrad": (_int, [ctypes.POINTER(_vp), ctypes.POINTER(_vp), ctypes.POINTER(_sz), _int, _int, _sz, _int,
+                                  _i64, _sz, _sz, _i64, _dbl, _int, _vp, _int, _sz, _vp, _sz, _vp]),
+    "dfcclPageCacheWorkspace": (_int, [_int, _int, ctypes.POINTER(_sz)]),
+    "dfcclPagesCopy": (_int, [_cache, _cache, _vp, _vp, _int, _vp]),
+    "dfcclPagesExtend": (_int, [_cache, _vp, _vp, _int, _vp]),
+    "dfcclPagesFork": (_int, [_cache, _vp, _vp, _int, _vp]),
+    "dfcclPagesFree": (_int, [_cache, _vp, _int, _vp]),
+    "dfcclPagesCompact": (_int, [_cache, _vp]),
     "dfcclGetStats": (_int, [_vp, ctypes.POINTER(Stats)]),
     "dfcclDumpState": (_int, [_vp]),
     "dfcclGetCollTiming": (_int, [_vp, _int, ctypes.POINTER(ctypes.c_uint64), ctypes.POINTER(ctypes.c_uint64)]),

@@ -1,0 +1,572 @@
+// Pages of a cache: copy, extend, fork, free, compact (dfcclPages* in ofccl.h).
+//
+// A cache is `npools` pools (keys and values of every layer, say) of the same number of pages that share one
+// numbering, and its bookkeeping in three arrays of 32-bit integers on the GPU: a reference count per page (0 = free),
+// a table row of page numbers per sequence, a length per sequence. Nothing else is kept, so there is no list of free
+// pages to go stale: whoever needs pages takes the lowest free ones, found by a scan of the counts.
+//
+// The contents are moved by the same code in copy, fork and compact, bound by HBM (each byte read once and written
+// once); the bookkeeping is a few integers per request, bound by the latency of its launches and scans.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "../../include/ofccl.h"
+#include "indexed_common.h"
+
+namespace dfccl {
+
+constexpr int kMoveThreads = 256;
+constexpr int kMoveWaves = kMoveThreads / 64;
+constexpr int kMaxPools = 64;  // per launch; more pools take several
+#ifndef DFCCL_SCAN_THREADS
+#define DFCCL_SCAN_THREADS 1024
+#endif
+constexpr int kScanThreads = DFCCL_SCAN_THREADS;
+constexpr int kScanWaves = kScanThreads / 64;
+constexpr int kScanPer = 4;  // counts a thread reads at once
+constexpr int kScanTile = kScanThreads * kScanPer;
+
+// The bookkeeping as the kernels see it.
+struct Books {
+  int32_t* refcounts;
+  int32_t* tables;
+  int32_t* lengths;
+  int32_t* report;  // may be null
+  int32_t pages, pageTokens, seqs, perSeq;
+};
+// Workspace: what one launch of a call hands to the next.
+struct PageScratch {
+  int32_t* owner;    // [seqs] first request that names the sequence
+  int32_t* request;  // [seqs] per request: number of its first new page among those found, or -1 if it is refused
+  int32_t* before;   // [seqs] per request: the sequence's (fork: the parent's) length before the call
+  int32_t* found;    // [pages] the lowest free pages (compact: the holes to fill), in order
+  int32_t* movers;   // [pages] compact: the pages that move, in order
+  int32_t* rank;     // [pages] compact: place among the movers
+  int32_t* counts;   // {pages found, pages that move}
+};
+
+__device__ __forceinline__ int32_t pagesOf(int32_t tokens, int32_t pageTokens) {
+  return tokens / pageTokens + (tokens % pageTokens != 0);
+}
+
+// ---- scan over the workgroup: exclusive prefix sum of v, and the total
+struct ScanShared {
+  int32_t wave[2][kScanWaves];
+};
+__device__ __forceinline__ int32_t blockScan(ScanShared& sh, int which, int32_t v, int32_t& total) {
+  const int lane = (int)(threadIdx.x & 63), wave = waveInBlock();
+  int32_t sum = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int32_t from = __shfl(sum, (lane - d) & 63);
+    if (lane >= d) sum += from;
+  }
+  if (lane == 63) sh.wave[which][wave] = sum;
+  __syncthreads();
+  int32_t before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kScanWaves; w++) {
+    const int32_t c = sh.wave[which][w];
+    if (w < wave) before += c;
+    total += c;
+  }
+  return before + sum - v;
+}
+
+// The numbers of a tile's pages that a thread looks at: kScanPer in a row.
+__device__ __forceinline__ void loadCounts(const Books& b, int64_t first, int32_t (&c)[kScanPer]) {
+#pragma unroll
+  for (int i = 0; i < kScanPer; i++) c[i] = first + i < b.pages ? b.refcounts[first + i] : 1;
+}
+
+// The lowest `most` free pages, in order, into found; returns how many there are (at most `most`). One workgroup.
+__device__ __forceinline__ int32_t findFree(ScanShared& sh, const Books& b, int32_t* found, int64_t most) {
+  int64_t have = 0;
+  int which = 0;
+  for (int64_t at = 0; at < b.pages && have < most; at += kScanTile, which ^= 1) {
+    const int64_t first = at + (int64_t)threadIdx.x * kScanPer;
+    int32_t c[kScanPer];
+    loadCounts(b, first, c);
+    int32_t mine = 0, total;
+#pragma unroll
+    for (int i = 0; i < kScanPer; i++) mine += c[i] == 0;
+    int64_t to = have + blockScan(sh, which, mine, total);
+#pragma unroll
+    for (int i = 0; i < kScanPer; i++)
+      if (c[i] == 0) {
+        if (to < most) found[to] = (int32_t)(first + i);
+        to++;
+      }
+    have += total;
+  }
+  return (int32_t)(have < most ? have : most);
+}
+
+// ---- requests: which are valid, and which new pages each gets. One workgroup.
+struct Requests {
+  const int32_t* a;  // extend: sequences; fork: parents
+  const int32_t* b;  // extend: lengths;   fork: children
+  int32_t n;
+};
+// extend: need = pages of the new length - pages of the old; fork: one page if the parent's last page is not full
+template <bool FORK>
+__global__ __launch_bounds__(kScanThreads) void assignKernel(Books b, PageScratch s, Requests q) {
+  struct Shared {
+    ScanShared scan;
+  };
+  DFCCL_WG_SHARED(Shared, sh);
+  const int tid = (int)threadIdx.x;
+  const int64_t most = (int64_t)b.perSeq * b.pageTokens;
+  // the first request that names a sequence (a fork: a child) has it; the others are refused
+  for (int32_t i = tid; i < q.n; i += kScanThreads) {
+    const int32_t seq = FORK ? q.b[i] : q.a[i];
+    if (seq >= 0 && seq < b.seqs) s.owner[seq] = 0x7fffffff;
+  }
+  __syncthreads();
+  for (int32_t i = tid; i < q.n; i += kScanThreads) {
+    const int32_t seq = FORK ? q.b[i] : q.a[i];
+    if (seq >= 0 && seq < b.seqs)
+      __hip_atomic_fetch_min(&s.owner[seq], i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  int64_t needed = 0;
+  int which = 0;
+  for (int32_t at = 0; at < q.n; at += kScanThreads, which ^= 1) {
+    const int32_t i = at + tid;
+    int32_t need = -1, before = 0;
+    if (i < q.n) {
+      const int32_t x = q.a[i], y = q.b[i];
+      const int32_t seq = FORK ? y : x;
+      if (seq >= 0 && seq < b.seqs && x >= 0 && x < b.seqs &&
+          __hip_atomic_load(&s.owner[seq], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == i) {
+        before = b.lengths[x];
+        const bool sound = before >= 0 && before <= most;
+        if constexpr (FORK) {
+          if (sound && b.lengths[y] == 0) need = before % b.pageTokens != 0;
+        } else {
+          if (sound && y >= before && y <= most) need = pagesOf(y, b.pageTokens) - pagesOf(before, b.pageTokens);
+        }
+      }
+      s.before[i] = before;
+    }
+    int32_t total;
+    const int32_t first = blockScan(sh.scan, which, need > 0 ? need : 0, total);
+    // (all needs together are at most seqs * perSeq, which the host keeps below 2^31)
+    if (i < q.n) s.request[i] = need < 0 ? -1 : (int32_t)needed + first;
+    needed += total;
+  }
+  __syncthreads();
+  const int32_t have = findFree(sh.scan, b, s.found, needed);
+  if (tid == 0) {
+    s.counts[0] = have;
+    if (b.report != nullptr) b.report[0] = 0;  // the launch that follows counts the refusals
+  }
+}
+
+__device__ __forceinline__ void refuse(const Books& b) {
+  if (b.report != nullptr) __hip_atomic_fetch_add(&b.report[0], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// One workgroup per request of an extend: the new entries, their counts, the length.
+__global__ __launch_bounds__(kMoveThreads) void extendKernel(Books b, PageScratch s, Requests q) {
+  for (int32_t i = (int32_t)blockIdx.x; i < q.n; i += (int32_t)gridDim.x) {
+    const int32_t first = s.request[i];
+    int32_t have = 0, want = 0, seq = 0, length = 0;
+    bool met = false;
+    if (first >= 0) {
+      seq = q.a[i];
+      length = q.b[i];
+      have = pagesOf(s.before[i], b.pageTokens);
+      want = pagesOf(length, b.pageTokens);
+      met = want == have || first + (want - have) <= s.counts[0];
+    }
+    if (!met) {
+      if (threadIdx.x == 0) refuse(b);
+      continue;
+    }
+    int32_t* row = b.tables + (size_t)seq * b.perSeq;
+    for (int32_t k = have + (int32_t)threadIdx.x; k < want; k += kMoveThreads) {
+      const int32_t page = s.found[first + k - have];
+      row[k] = page;
+      b.refcounts[page] = 1;
+    }
+    if (threadIdx.x == 0) b.lengths[seq] = length;
+  }
+}
+
+// ---- contents
+
+struct PoolSet {
+  char* to[kMaxPools];
+  const char* from[kMaxPools];
+  int32_t npools;
+  uint32_t parts;      // per page
+  uint32_t lastBytes;  // of a page's last part
+  size_t pageBytes;
+};
+constexpr int kPartLoads = 4;                                     // 16-byte loads a lane has in flight
+constexpr uint32_t kPartBytes = 64 * 16 * kPartLoads;             // what one wave moves at a time
+
+// one part of a page, by one wave
+__device__ __forceinline__ void movePart(const char* from, char* to, uint32_t bytes, uint32_t lane) {
+  if (bytes == kPartBytes) {
+    u32x4 v[kPartLoads];
+#pragma unroll
+    for (int u = 0; u < kPartLoads; u++) v[u] = load16<1>(from + (u * 64 + lane) * 16);
+#pragma unroll
+    for (int u = 0; u < kPartLoads; u++) store16<1>(to + (u * 64 + lane) * 16, v[u]);
+    return;
+  }
+  const uint32_t packs = bytes / 16;
+  for (uint32_t p = lane; p < packs; p += 64) store16<1>(to + p * 16, load16<1>(from + p * 16));
+  for (uint32_t i = packs * 16 + lane; i < bytes; i += 64)
+    ((DFCCL_GLOBAL char*)to)[i] = ((const DFCCL_GLOBAL char*)from)[i];
+}
+// item = (pair, pool, part) of a move, numbered so that neighbours touch neighbouring memory
+__device__ __forceinline__ void moveItem(const PoolSet& p, int32_t src, int32_t dst, uint32_t inPair, int lane) {
+  const uint32_t pool = inPair / p.parts, part = inPair % p.parts;
+  const size_t at = (size_t)part * kPartBytes;
+  // (the last part's size comes from the host: the minimum of two 64-bit sizes that are the same in every lane is
+  // compiled into a vector compare whose result the scalar select that follows does not read)
+  const uint32_t bytes = part + 1 == p.parts ? p.lastBytes : kPartBytes;
+  movePart(p.from[pool] + (size_t)src * p.pageBytes + at, p.to[pool] + (size_t)dst * p.pageBytes + at, bytes, (uint32_t)lane);
+}
+
+__global__ __launch_bounds__(kMoveThreads) void copyKernel(PoolSet p, const int32_t* srcPages, const int32_t* dstPages,
+                                                           int32_t n, int32_t srcTotal, int32_t dstTotal) {
+  const int lane = (int)(threadIdx.x & 63);
+  const uint32_t perPair = (uint32_t)p.npools * p.parts;
+  const uint64_t items = (uint64_t)n * perPair;
+  for (uint64_t item = (uint64_t)blockIdx.x * kMoveWaves + waveInBlock(); item < items;
+       item += (uint64_t)gridDim.x * kMoveWaves) {
+    const uint32_t i = (uint32_t)(item / perPair);
+    const int32_t src = uniform(srcPages[i]), dst = uniform(dstPages[i]);
+    if (src < 0 || src >= srcTotal || dst < 0 || dst >= dstTotal) continue;
+    moveItem(p, src, dst, (uint32_t)(item % perPair), lane);
+  }
+}
+
+// Fork, the tables: one workgroup per request. The child's whole pages are the parent's; a last page that is not full
+// is the child's own, its contents copied by forkMoveKernel (from the table rows, which this kernel's launch precedes).
+__global__ __launch_bounds__(kMoveThreads) void forkKernel(Books b, PageScratch s, Requests q) {
+  for (int32_t i = (int32_t)blockIdx.x; i < q.n; i += (int32_t)gridDim.x) {
+    const int32_t first = s.request[i];
+    const int32_t before = s.before[i];
+    const int32_t whole = before / b.pageTokens, need = before % b.pageTokens != 0;
+    if (first < 0 || (need != 0 && first >= s.counts[0])) {
+      if (threadIdx.x == 0) refuse(b);
+      continue;
+    }
+    const int32_t parent = q.a[i], child = q.b[i];
+    const int32_t* from = b.tables + (size_t)parent * b.perSeq;
+    int32_t* to = b.tables + (size_t)child * b.perSeq;
+    for (int32_t k = (int32_t)threadIdx.x; k < whole; k += kMoveThreads) {
+      const int32_t page = from[k];
+      to[k] = page;
+      if (page >= 0 && page < b.pages) __hip_atomic_fetch_add(&b.refcounts[page], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if (threadIdx.x == 0) {
+      if (need != 0) {
+        const int32_t page = s.found[first];
+        to[whole] = page;
+        b.refcounts[page] = 1;
+      }
+      b.lengths[child] = before;
+    }
+  }
+}
+__global__ __launch_bounds__(kMoveThreads) void forkMoveKernel(Books b, PageScratch s, Requests q, PoolSet p) {
+  const int lane = (int)(threadIdx.x & 63);
+  const uint32_t perPair = (uint32_t)p.npools * p.parts;
+  const uint64_t items = (uint64_t)q.n * perPair;
+  for (uint64_t item = (uint64_t)blockIdx.x * kMoveWaves + waveInBlock(); item < items;
+       item += (uint64_t)gridDim.x * kMoveWaves) {
+    const uint32_t i = (uint32_t)(item / perPair);
+    const int32_t first = uniform(s.request[i]), before = uniform(s.before[i]);
+    if (first < 0 || before % b.pageTokens == 0 || first >= uniform(s.counts[0])) continue;
+    const int32_t src = uniform(b.tables[(size_t)uniform(q.a[i]) * b.perSeq + before / b.pageTokens]);
+    if (src < 0 || src >= b.pages) continue;
+    moveItem(p, src, uniform(s.found[first]), (uint32_t)(item % perPair), lane);
+  }
+}
+
+// Free: one workgroup per sequence. Whoever takes the length out frees the pages, so a sequence that is listed
+// twice is freed once.
+__global__ __launch_bounds__(kMoveThreads) void freeKernel(Books b, const int32_t* seqs, int32_t n) {
+  struct Shared {
+    int32_t length;
+  };
+  DFCCL_WG_SHARED(Shared, sh);
+  for (int32_t i = (int32_t)blockIdx.x; i < n; i += (int32_t)gridDim.x) {
+    const int32_t seq = seqs[i];
+    if (threadIdx.x == 0)
+      sh.length = seq >= 0 && seq < b.seqs
+                      ? __hip_atomic_exchange(&b.lengths[seq], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
+                      : 0;
+    __syncthreads();
+    const int32_t length = sh.length;
+    if (length > 0) {
+      int32_t used = pagesOf(length, b.pageTokens);
+      if (used > b.perSeq) used = b.perSeq;
+      int32_t* row = b.tables + (size_t)seq * b.perSeq;
+      for (int32_t k = (int32_t)threadIdx.x; k < used; k += kMoveThreads) {
+        const int32_t page = row[k];
+        row[k] = -1;
+        if (page >= 0 && page < b.pages)
+          __hip_atomic_fetch_add(&b.refcounts[page], -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Compact, the plan: with L pages live, the k-th live page at or above L goes to the k-th free page below L. Sources
+// and destinations are disjoint, so all of them can move at once, and no plan moves fewer pages. One workgroup.
+__global__ __launch_bounds__(kScanThreads) void compactPlanKernel(Books b, PageScratch s) {
+  struct Shared {
+    ScanShared scan;
+  };
+  DFCCL_WG_SHARED(Shared, sh);
+  int32_t live = 0;
+  int which = 0;
+  for (int64_t at = 0; at < b.pages; at += kScanTile, which ^= 1) {
+    int32_t c[kScanPer], mine = 0, total;
+    loadCounts(b, at + (int64_t)threadIdx.x * kScanPer, c);
+#pragma unroll
+    for (int i = 0; i < kScanPer; i++) mine += c[i] > 0 && at + (int64_t)threadIdx.x * kScanPer + i < b.pages;
+    (void)blockScan(sh.scan, which, mine, total);
+    live += total;
+  }
+  int32_t holes = 0, movers = 0;
+  for (int64_t at = 0; at < b.pages; at += kScanTile) {
+    const int64_t first = at + (int64_t)threadIdx.x * kScanPer;
+    int32_t c[kScanPer], hole = 0, mover = 0, totalHoles, totalMovers;
+    loadCounts(b, first, c);
+#pragma unroll
+    for (int i = 0; i < kScanPer; i++) {
+      hole += first + i < live && c[i] <= 0;
+      mover += first + i >= live && first + i < b.pages && c[i] > 0;
+    }
+    __syncthreads();  // (the totals of the round before have been read)
+    int32_t h = holes + blockScan(sh.scan, 0, hole, totalHoles);
+    int32_t m = movers + blockScan(sh.scan, 1, mover, totalMovers);
+#pragma unroll
+    for (int i = 0; i < kScanPer; i++) {
+      if (first + i < live && c[i] <= 0) s.found[h++] = (int32_t)(first + i);
+      if (first + i >= live && first + i < b.pages && c[i] > 0) {
+        s.rank[first + i] = m;
+        s.movers[m++] = (int32_t)(first + i);
+      }
+    }
+    holes += totalHoles;
+    movers += totalMovers;
+  }
+  if (threadIdx.x == 0) {
+    s.counts[0] = holes;
+    s.counts[1] = movers;  // (as many as holes)
+    if (b.report != nullptr) {
+      b.report[1] = movers;
+      b.report[2] = live;
+    }
+  }
+}
+__global__ __launch_bounds__(kMoveThreads) void compactMoveKernel(Books b, PageScratch s, PoolSet p) {
+  const int lane = (int)(threadIdx.x & 63);
+  const uint32_t perPair = (uint32_t)p.npools * p.parts;
+  const uint64_t items = (uint64_t)uniform(s.counts[1]) * perPair;
+  for (uint64_t item = (uint64_t)blockIdx.x * kMoveWaves + waveInBlock(); item < items;
+       item += (uint64_t)gridDim.x * kMoveWaves) {
+    const uint32_t i = (uint32_t)(item / perPair);
+    moveItem(p, uniform(s.movers[i]), uniform(s.found[i]), (uint32_t)(item % perPair), lane);
+  }
+}
+// Compact, the bookkeeping: table entries follow the moves, and the counts move with their pages.
+__global__ __launch_bounds__(kMoveThreads) void compactBooksKernel(Books b, PageScratch s) {
+  const int32_t moves = s.counts[1];
+  for (int32_t i = (int32_t)(blockIdx.x * kMoveThreads + threadIdx.x); i < moves; i += (int32_t)(gridDim.x * kMoveThreads)) {
+    const int32_t from = s.movers[i], to = s.found[i];
+    b.refcounts[to] = b.refcounts[from];
+    b.refcounts[from] = 0;
+  }
+  for (int32_t seq = (int32_t)blockIdx.x; seq < b.seqs; seq += (int32_t)gridDim.x) {
+    const int32_t length = b.lengths[seq];
+    if (length <= 0) continue;
+    int32_t used = pagesOf(length, b.pageTokens);
+    if (used > b.perSeq) used = b.perSeq;
+    int32_t* row = b.tables + (size_t)seq * b.perSeq;
+    for (int32_t k = (int32_t)threadIdx.x; k < used; k += kMoveThreads) {
+      const int32_t page = row[k];
+      if (page < 0 || page >= b.pages) continue;
+      const int32_t r = s.rank[page];  // (left over from anywhere for a page that does not move)
+      if (r >= 0 && r < moves && s.movers[r] == page) row[k] = s.found[r];
+    }
+  }
+}
+
+// ---- host
+
+struct PagePlan {
+  size_t owner, request, before, found, movers, rank, counts, bytes;
+};
+static PagePlan planPages(int64_t pages, int64_t seqs) {
+  PagePlan p{};
+  size_t at = 0;
+  auto take = [&at](int64_t ints) {
+    const size_t here = at;
+    at += ((size_t)ints * 4 + 255) & ~(size_t)255;
+    return here;
+  };
+  p.owner = take(seqs);
+  p.request = take(seqs);
+  p.before = take(seqs);
+  p.found = take(pages);
+  p.movers = take(pages);
+  p.rank = take(pages);
+  p.counts = take(4);
+  p.bytes = at;
+  return p;
+}
+
+static bool soundPools(const dfcclPageCache* c) {
+  if (c == nullptr || c->structBytes < sizeof(dfcclPageCache)) return false;
+  if (c->pages < 1 || c->npools < 1 || c->pageBytes == 0 || c->pools == nullptr) return false;
+  for (int i = 0; i < c->npools; i++)
+    if (c->pools[i] == nullptr) return false;
+  return true;
+}
+static bool soundCache(const dfcclPageCache* c) {
+  if (!soundPools(c)) return false;
+  if (c->pageTokens < 1 || c->sequences < 1 || c->pagesPerSequence < 1) return false;
+  // entries and lengths are 32-bit integers
+  if ((int64_t)c->sequences * c->pagesPerSequence > 0x7fffffffll) return false;
+  if ((int64_t)c->pagesPerSequence * c->pageTokens > 0x7fffffffll) return false;
+  if (c->refcounts == nullptr || c->tables == nullptr || c->lengths == nullptr || c->workspace == nullptr) return false;
+  return c->workspaceBytes >= planPages(c->pages, c->sequences).bytes && ((uintptr_t)c->workspace & 3u) == 0;
+}
+static Books booksOf(const dfcclPageCache* c) {
+  Books b{};
+  b.refcounts = c->refcounts;
+  b.tables = c->tables;
+  b.lengths = c->lengths;
+  b.report = c->report;
+  b.pages = c->pages;
+  b.pageTokens = c->pageTokens;
+  b.seqs = c->sequences;
+  b.perSeq = c->pagesPerSequence;
+  return b;
+}
+static PageScratch scratchOf(const dfcclPageCache* c) {
+  const PagePlan p = planPages(c->pages, c->sequences);
+  char* ws = (char*)c->workspace;
+  PageScratch s{};
+  s.owner = (int32_t*)(ws + p.owner);
+  s.request = (int32_t*)(ws + p.request);
+  s.before = (int32_t*)(ws + p.before);
+  s.found = (int32_t*)(ws + p.found);
+  s.movers = (int32_t*)(ws + p.movers);
+  s.rank = (int32_t*)(ws + p.rank);
+  s.counts = (int32_t*)(ws + p.counts);
+  return s;
+}
+static PoolSet poolSet(const dfcclPageCache* to, const dfcclPageCache* from, int first) {
+  PoolSet p{};
+  p.npools = std::min(kMaxPools, to->npools - first);
+  for (int i = 0; i < p.npools; i++) {
+    p.to[i] = (char*)to->pools[first + i];
+    p.from[i] = (const char*)from->pools[first + i];
+  }
+  p.pageBytes = to->pageBytes;
+  p.parts = (uint32_t)((to->pageBytes + kPartBytes - 1) / kPartBytes);
+  p.lastBytes = (uint32_t)(to->pageBytes - (size_t)(p.parts - 1) * kPartBytes);
+  return p;
+}
+constexpr uint64_t kMaxMoveGrid = 1u << 22;
+static unsigned moveGrid(uint64_t items) {
+  return (unsigned)std::max<uint64_t>(1, std::min<uint64_t>((items + kMoveWaves - 1) / kMoveWaves, kMaxMoveGrid));
+}
+static ncclResult_t launched() { return hipGetLastError() == hipSuccess ? ncclSuccess : ncclUnhandledCudaError; }
+// a page's parts over a launch's pools are counted in 32 bits
+static bool soundPage(const dfcclPageCache* c) { return c->pageBytes <= ((size_t)1 << 36); }  // (2^24 parts, 64 pools)
+
+}  // namespace dfccl
+
+using namespace dfccl;
+
+#define DFCCL_API extern "C" __attribute__((visibility("default")))
+
+DFCCL_API ncclResult_t dfcclPageCacheWorkspace(int pages, int sequences, size_t* bytes) {
+  if (pages < 1 || sequences < 1 || bytes == nullptr) return ncclInvalidArgument;
+  *bytes = planPages(pages, sequences).bytes;
+  return ncclSuccess;
+}
+
+DFCCL_API ncclResult_t dfcclPagesCopy(const dfcclPageCache* to, const dfcclPageCache* from, const int32_t* srcPages,
+                                      const int32_t* dstPages, int n, void* stream) {
+  if (!soundPools(to) || !soundPools(from) || !soundPage(to)) return ncclInvalidArgument;
+  if (to->npools != from->npools || to->pageBytes != from->pageBytes || n < 0) return ncclInvalidArgument;
+  if (n == 0) return ncclSuccess;
+  if (srcPages == nullptr || dstPages == nullptr) return ncclInvalidArgument;
+  for (int first = 0; first < to->npools; first += kMaxPools) {
+    const PoolSet p = poolSet(to, from, first);
+    DFCCL_LAUNCH_BLOCKS(copyKernel, moveGrid((uint64_t)n * p.npools * p.parts), kMoveThreads, (hipStream_t)stream, p, srcPages,
+                        dstPages, n, from->pages, to->pages);
+  }
+  return launched();
+}
+
+DFCCL_API ncclResult_t dfcclPagesExtend(const dfcclPageCache* c, const int32_t* sequences, const int32_t* lengths, int n,
+                                        void* stream) {
+  if (!soundCache(c) || n < 0 || n > c->sequences) return ncclInvalidArgument;
+  if (n > 0 && (sequences == nullptr || lengths == nullptr)) return ncclInvalidArgument;
+  const Books b = booksOf(c);
+  const hipStream_t st = (hipStream_t)stream;
+  const PageScratch s = scratchOf(c);
+  const Requests q{sequences, lengths, n};
+  DFCCL_LAUNCH_BLOCKS(assignKernel<false>, 1, kScanThreads, st, b, s, q);
+  if (n > 0) DFCCL_LAUNCH_BLOCKS(extendKernel, (unsigned)n, kMoveThreads, st, b, s, q);
+  return launched();
+}
+
+DFCCL_API ncclResult_t dfcclPagesFork(const dfcclPageCache* c, const int32_t* parents, const int32_t* children, int n,
+                                      void* stream) {
+  if (!soundCache(c) || !soundPage(c) || n < 0 || n > c->sequences) return ncclInvalidArgument;
+  if (n > 0 && (parents == nullptr || children == nullptr)) return ncclInvalidArgument;
+  const Books b = booksOf(c);
+  const hipStream_t st = (hipStream_t)stream;
+  const PageScratch s = scratchOf(c);
+  const Requests q{parents, children, n};
+  DFCCL_LAUNCH_BLOCKS(assignKernel<true>, 1, kScanThreads, st, b, s, q);
+  if (n > 0) {
+    DFCCL_LAUNCH_BLOCKS(forkKernel, (unsigned)n, kMoveThreads, st, b, s, q);
+    for (int first = 0; first < c->npools; first += kMaxPools) {
+      const PoolSet p = poolSet(c, c, first);
+      DFCCL_LAUNCH_BLOCKS(forkMoveKernel, moveGrid((uint64_t)n * p.npools * p.parts), kMoveThreads, st, b, s, q, p);
+    }
+  }
+  return launched();
+}
+
+DFCCL_API ncclResult_t dfcclPagesFree(const dfcclPageCache* c, const int32_t* sequences, int n, void* stream) {
+  if (!soundCache(c) || n < 0 || (n > 0 && sequences == nullptr)) return ncclInvalidArgument;
+  if (n == 0) return ncclSuccess;
+  DFCCL_LAUNCH_BLOCKS(freeKernel, (unsigned)std::min(n, 1 << 20), kMoveThreads, (hipStream_t)stream, booksOf(c), sequences, n);
+  return launched();
+}
+
+DFCCL_API ncclResult_t dfcclPagesCompact(const dfcclPageCache* c, void* stream) {
+  if (!soundCache(c) || !soundPage(c)) return ncclInvalidArgument;
+  const Books b = booksOf(c);
+  const PageScratch s = scratchOf(c);
+  const hipStream_t st = (hipStream_t)stream;
+  DFCCL_LAUNCH_BLOCKS(compactPlanKernel, 1, kScanThreads, st, b, s);
+  for (int first = 0; first < c->npools; first += kMaxPools) {
+    const PoolSet p = poolSet(c, c, first);
+    // how many pages move is known on the GPU only: at most half of them
+    const uint64_t most = (uint64_t)(c->pages / 2) * p.npools * p.parts;
+    DFCCL_LAUNCH_BLOCKS(compactMoveKernel, std::min(moveGrid(most), 2048u), kMoveThreads, st, b, s, p);
+  }
+  DFCCL_LAUNCH_BLOCKS(compactBooksKernel, (unsigned)std::min(c->sequences, 2048), kMoveThreads, st, b, s);
+  return launched();
+}

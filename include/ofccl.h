@@ -189,6 +189,107 @@ ncclResult_t ofcclRunAllGather(const void* sendbuff, void* recvbuff, int collId,
 ncclResult_t dfcclReduceCopy(const void* const* srcs, int nsrcs, void* dst, size_t count, ncclDataType_t datatype,
                              ncclRedOp_t op, size_t chunkBytes, void* stream);
 
+/* ---- rows of a table through an index --------------------------------------
+ * The two things the library does to dense buffers, copying and summing, for
+ * rows that are named by token ids on the device: the embedding lookup and its
+ * gradient.  No counterpart in the reference.  `table` may be the whole table
+ * or one rank's piece of the vocabulary, `rows` rows that begin with id
+ * firstRow (>= 0); an id outside the piece names no row.  Tables, outputs and
+ * gradients are ncclFloat32, ncclFloat16 or ncclBfloat16, each of its own type
+ * and aligned to it; ids are ncclInt32 or ncclInt64.  Strides are in elements,
+ * from row to row, at least `width`.  Up to 2^31-1 tokens, rows and columns.
+ * Asynchronous on `stream`, allocate nothing, may be captured into a graph. */
+
+/* out[t,:] = scale * table[id_t - firstRow,:], computed in fp32 and rounded
+ * once; zeros for an id that names no row, so that the sum of the ranks'
+ * outputs over the pieces (an all-reduce) is the lookup in the whole table. */
+ncclResult_t dfcclEmbeddingLookup(const void* table, ncclDataType_t tableType, size_t rows, size_t tableStride,
+                                  int64_t firstRow, const void* ids, ncclDataType_t idType, size_t tokens, size_t width,
+                                  double scale, void* out, ncclDataType_t outType, size_t outStride, void* stream);
+
+/* tableGrad[v,:] = scale * the sum of grads[r][t,:] over all tokens t of all
+ * sources r (1..8: the ranks' batches, tokens[r] < 2^28 each) whose id names
+ * row v.  Tokens whose id is paddingId (negative: no such id) are left out.
+ * Summed in fp32 in an order that depends on the ids alone (source by source,
+ * token by token, long runs in blocks): the same call gives the same bits.
+ * accumulate = 0 writes every row (zeros where no token names one);
+ * accumulate = 1 adds to the rows that tokens name and touches no other.
+ * grads, ids and tokens are host arrays of nsrcs entries; tokens[r] may be 0.
+ * `workspace` is device memory (16-byte aligned) of at least the bytes that
+ * dfcclEmbeddingGradWorkspace gives for the same sizes; it holds nothing
+ * between calls, but two calls that may run at the same time need one each. */
+ncclResult_t dfcclEmbeddingGradWorkspace(int nsrcs, const size_t* tokens, size_t rows, size_t width, size_t* bytes);
+ncclResult_t dfcclEmbeddingGrad(const void* const* grads, const void* const* ids, const size_t* tokens, int nsrcs,
+                                ncclDataType_t gradType, size_t gradStride, ncclDataType_t idType, int64_t firstRow,
+                                size_t rows, size_t width, int64_t paddingId, double scale, int accumulate,
+                                void* tableGrad, ncclDataType_t tableType, size_t tableStride, void* workspace,
+                                size_t workspaceBytes, void* stream);
+
+/* ---- pages of a cache -------------------------------------------------------
+ * A rank's cache of keys and values: `npools` pools (one for each layer's keys
+ * and one for its values, say) of `pages` pages of `pageBytes` bytes, back to
+ * back, that share one numbering.  Which sequence has which pages is kept on
+ * the device in 32-bit integers that the caller owns and may read:
+ *   refcounts[pages]                      how many table entries name a page; 0: it is free
+ *   tables[sequences][pagesPerSequence]   the pages of a sequence, in order; -1 behind them
+ *   lengths[sequences]                    tokens; ceil(length / pageTokens) entries are in use
+ * An empty cache is refcounts = 0, tables = -1, lengths = 0.  No counterpart
+ * in the reference.  All calls are asynchronous on `stream`, allocate nothing
+ * and may be captured into a graph; calls that change one cache have to follow
+ * each other (one stream, or events between streams).  Lists of sequences,
+ * pages and lengths are int32 arrays on the device.  What a list asks for and
+ * cannot have (a sequence out of range, no page free) is refused there, as the
+ * calls say; table entries and list entries out of range are never followed. */
+typedef struct {
+  uint64_t structBytes;       /* sizeof(dfcclPageCache) */
+  void* const* pools;         /* host array of npools device pointers */
+  size_t pageBytes;           /* of one page in one pool */
+  int npools;
+  int pages;
+  int pageTokens;
+  int sequences;
+  int pagesPerSequence;
+  int32_t* refcounts;
+  int32_t* tables;
+  int32_t* lengths;
+  int32_t* report;            /* device, 3 integers, or NULL: requests refused by the last Extend or Fork; pages moved
+                                 and pages live at the last Compact */
+  void* workspace;            /* device; dfcclPageCacheWorkspace says how much; holds nothing between calls */
+  size_t workspaceBytes;
+} dfcclPageCache;
+ncclResult_t dfcclPageCacheWorkspace(int pages, int sequences, size_t* bytes);
+
+/* Copies the contents of page srcPages[i] of `from` to page dstPages[i] of `to`
+ * in every pool, for n pairs; the bookkeeping of neither is read or written
+ * (refcounts, tables, lengths and workspace may be NULL here).  The two may be
+ * the same cache, or two ranks' of the same npools and pageBytes.  Pairs with
+ * a page out of range are left out.  No destination may appear twice, or as a
+ * source of the same pool: the order of the pairs is not defined. */
+ncclResult_t dfcclPagesCopy(const dfcclPageCache* to, const dfcclPageCache* from, const int32_t* srcPages,
+                            const int32_t* dstPages, int n, void* stream);
+/* Sequence sequences[i] grows to lengths[i] tokens.  New entries get the lowest
+ * free pages, in the order of the requests, until the free pages run out
+ * (behind a request that finds too few, every one that needs a page is refused).
+ * Refused whole: a sequence out of range or listed before, a length below the
+ * present one or above what a table row holds, more pages than are left.
+ * n <= the cache's sequences (the same for Fork). */
+ncclResult_t dfcclPagesExtend(const dfcclPageCache* cache, const int32_t* sequences, const int32_t* lengths, int n,
+                              void* stream);
+/* Sequence children[i] (empty) becomes a copy of parents[i] as it is before the
+ * call: full pages are shared, a last page that is not full is copied to the
+ * lowest free page, so that both can go on writing (free pages are handed out
+ * as by Extend).  Refused whole: a sequence
+ * out of range, a child that is not empty or listed before, no page left. */
+ncclResult_t dfcclPagesFork(const dfcclPageCache* cache, const int32_t* parents, const int32_t* children, int n,
+                            void* stream);
+/* The listed sequences become empty and give up their pages.  Empty ones, ones
+ * out of range and further mentions of a sequence are left alone. */
+ncclResult_t dfcclPagesFree(const dfcclPageCache* cache, const int32_t* sequences, int n, void* stream);
+/* Moves pages until the live ones have the lowest numbers: with L of them the
+ * k-th live page from L on goes to the k-th free page below L, in every pool,
+ * and counts and table entries follow. */
+ncclResult_t dfcclPagesCompact(const dfcclPageCache* cache, void* stream);
+
 /* ---- introspection (reference: counters printed at final quit,
  * src/include/collectives_ofccl.h:173-179, enqueue_ofccl_dev.cu:1148) ------ */
 

@@ -153,6 +153,35 @@ void launch(Stream* s, unsigned grid, unsigned block, std::function<void()> body
   gJobs.push_back(job);
 }
 
+void launchBlocks(Stream* s, unsigned grid, unsigned block, std::function<void()> body) {
+  if (s == nullptr) s = &gNullStream;
+  std::shared_ptr<Job> prev;
+  {
+    std::lock_guard<std::mutex> lk(s->mu);
+    prev = s->last;
+  }
+  if (prev) prev->join();
+  constexpr unsigned kAtOnce = 4;
+  for (unsigned at = 0; at < grid; at += kAtOnce) {
+    const unsigned n = grid - at < kAtOnce ? grid - at : kAtOnce;
+    std::shared_ptr<Job> job;
+    Stream own;
+    launch(&own, n, block, [=]() {
+      tls.bIdx = Dim3(at + tls.bIdx.x);
+      tls.gDim = Dim3(grid);
+      body();
+    });
+    job = own.last;
+    job->join();
+    std::lock_guard<std::mutex> lk(gJobsMu);  // (thousands of such launches: their workgroups' memory goes at once)
+    for (size_t j = gJobs.size(); j-- > 0;)
+      if (gJobs[j] == job) {
+        gJobs.erase(gJobs.begin() + (long)j);
+        break;
+      }
+  }
+}
+
 // Where every thread of every launch that has not ended is (for a run that has stopped moving).
 void dumpThreads(FILE* f) {
   std::lock_guard<std::mutex> lk(gJobsMu);

@@ -158,6 +158,8 @@ struct Stream;  // launches in order
 struct Event;
 
 void launch(Stream* s, unsigned grid, unsigned block, std::function<void()> body);
+// a launch whose workgroups do not wait for each other: a few of them at a time, ended when it returns
+void launchBlocks(Stream* s, unsigned grid, unsigned block, std::function<void()> body);
 
 }  // namespace emul
 
@@ -191,11 +193,14 @@ typedef ::emul::Dim3 dim3;
 #define __builtin_amdgcn_readlane(x, srcLane) ::emul::shflFrom((x), (srcLane), __LINE__)
 #define __builtin_amdgcn_fence(order, scope) __atomic_thread_fence(__ATOMIC_SEQ_CST)
 #define __builtin_amdgcn_s_sleep(n) sched_yield()
+#define __HIP_MEMORY_SCOPE_WORKGROUP 0
 #define __HIP_MEMORY_SCOPE_AGENT 0
 #define __HIP_MEMORY_SCOPE_SYSTEM 0
 #define __hip_atomic_load(p, order, scope) __atomic_load_n((p), __ATOMIC_SEQ_CST)
 #define __hip_atomic_store(p, v, order, scope) __atomic_store_n((p), (v), __ATOMIC_SEQ_CST)
 #define __hip_atomic_fetch_add(p, v, order, scope) __atomic_fetch_add((p), (v), __ATOMIC_SEQ_CST)
+#define __hip_atomic_exchange(p, v, order, scope) __atomic_exchange_n((p), (v), __ATOMIC_SEQ_CST)
+#define __hip_atomic_fetch_min(p, v, order, scope) __atomic_fetch_min((p), (v), __ATOMIC_SEQ_CST)
 
 inline uint64_t wall_clock64() {  // 100 MHz
   timespec ts;
@@ -249,3 +254,8 @@ template <typename K, typename... Args>
 inline void hipLaunchKernelGGL(K kernel, dim3 grid, dim3 block, size_t, hipStream_t stream, Args... args) {
   emul::launch(stream, grid.x, block.x, [=]() { kernel(args...); });
 }
+template <typename K, typename... Args>
+inline void emulLaunchBlocks(K kernel, unsigned grid, unsigned block, hipStream_t stream, Args... args) {
+  emul::launchBlocks(stream, grid, block, [=]() { kernel(args...); });
+}
+#define DFCCL_LAUNCH_BLOCKS(kernel, grid, block, stream, ...) emulLaunchBlocks(kernel, grid, block, stream, __VA_ARGS__)
