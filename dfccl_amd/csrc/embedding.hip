@@ -117,9 +117,11 @@ static LookupKernel pickLookup(int in, int out) {
 // 2. Chunks. The sorted list is cut into chunks of kChunk. A chunk that lies within one row's run is summed by a
 //    wave of its own into fp32 scratch, and so are kChunk such chunks: a row that many tokens share (padding that
 //    counts, frequent words) is summed by many waves, and again in a fixed order.
-// 3. Rows. A wave per row piece adds up its run: single tokens up to the first whole chunk, whole chunks' (and
-//    chunks of chunks') sums, single tokens after the last. Each row is written once; a row without tokens gets
-//    zeros (or is left alone when accumulating).
+// 3. Rows. A wave per sorted position and row piece goes on where its position begins a run: single tokens up to the
+//    first whole chunk, whole chunks' (and chunks of chunks') sums, single tokens after the last.
+// Without accumulation the rows that no token names have to become zeros. That is most of the table and most of the
+// bytes, and it needs nothing of the sort: all rows are cleared by additional workgroups of the launches of 1. and 2.,
+// which leave most of the chip idle, and the named rows are written over afterwards.
 
 constexpr int kChunk = 32;
 constexpr int kMaxDigitBits = 10;
@@ -136,21 +138,50 @@ struct GradArgs {
   int64_t firstRow, paddingId;
   uint32_t rows, width, pieces, n;
   float scale;
+  bool accumulate, chunked, supered;  // (whether there are sums of chunks, and of chunks of chunks)
   char* table;
   // workspace
   uint32_t* keys[2];
   uint32_t* pays[2];
-  uint32_t* hist;      // [tiles][bins]
-  int32_t* rowBegin;   // position of a row's first token in the sorted list, -1 without one
-  uint32_t* rowEnd;    // behind its last
-  float* chunkSums;    // [n / kChunk][widthPad]
-  float* superSums;    // [n / kChunk^2][widthPad]
-  uint32_t widthPad;   // width rounded up to kVec
+  uint32_t* hist;     // [tiles][bins]
+  float* chunkSums;   // [n / kChunk][widthPad]
+  float* superSums;   // [n / kChunk^2][widthPad]
+  uint32_t widthPad;  // width rounded up to kVec
 };
 
 struct SortPass {
   int from, shift, bits, tiles;  // keys[from] -> keys[from ^ 1]
 };
+
+// A share of the clearing of the table: parts [begin, end) of rows of `bytes` bytes, each row in `parts` parts.
+// (A table without gaps between its rows is one long row.)
+struct Clear {
+  char* at;
+  size_t stride;
+  uint64_t bytes, parts, begin, end;
+  uint32_t firstBlock;  // the launch's workgroups from here on clear
+};
+constexpr int kClearStores = 4;
+constexpr uint32_t kClearBytes = 64 * 16 * kClearStores;  // of a part
+constexpr unsigned kClearWavesPerCu = 16;
+
+__device__ __forceinline__ void clearShare(const Clear& c, uint32_t waves) {
+  const uint32_t lane = threadIdx.x & 63, blocks = gridDim.x - c.firstBlock;
+  const u32x4 zero = {0, 0, 0, 0};
+  for (uint64_t i = c.begin + (uint64_t)(blockIdx.x - c.firstBlock) * waves + (uint32_t)waveInBlock(); i < c.end;
+       i += (uint64_t)blocks * waves) {
+    const uint64_t row = i / c.parts, part = i % c.parts;
+    char* to = c.at + row * c.stride + part * kClearBytes;
+    if (part + 1 < c.parts) {
+#pragma unroll
+      for (int u = 0; u < kClearStores; u++) store16<2>(to + (u * 64 + lane) * 16, zero);
+    } else {  // a row's last part, 1 .. kClearBytes bytes, an even number
+      const uint32_t left = (uint32_t)(c.bytes - part * kClearBytes);
+      for (uint32_t p = lane; p < left / 16; p += 64) store16<2>(to + p * 16, zero);
+      for (uint32_t p = left / 16 * 8 + lane; p < left / 2; p += 64) storeElem<2>(to, p, 0);
+    }
+  }
+}
 
 __device__ __forceinline__ void keyOfToken(const GradArgs& a, uint32_t pos, uint32_t& key, uint32_t& pay) {
   int r = 0;
@@ -169,26 +200,140 @@ __device__ __forceinline__ void keyOfToken(const GradArgs& a, uint32_t pos, uint
   pay = ((uint32_t)r << kSrcShift) | t;
 }
 
+// A strip's 64 keys of one wave: every lane's rank among the strip's keys of its digit, found with a ballot per bit,
+// and their number (`same`, a mask). Lanes without a key are in no mask.
+__device__ __forceinline__ uint64_t sameDigit(uint32_t digit, int bits, bool valid) {
+  uint64_t same = __ballot(valid);
+  for (int b = 0; b < bits; b++) {
+    const bool one = (digit >> b) & 1u;
+    const uint64_t ones = __ballot(one);
+    same &= one ? ones : ~ones;
+  }
+  return same;
+}
+// The rank of a strip's keys among the wave's keys of the same digit so far, whose counts are kept in LDS.
+__device__ __forceinline__ uint32_t rankInWave(uint32_t* count, uint32_t digit, int bits, bool valid, int lane) {
+  const uint64_t same = sameDigit(digit, bits, valid);
+  const uint64_t before = same & ((1ull << lane) - 1);
+  const uint32_t old = count[digit];
+  DFCCL_WAVE_LDS_SYNC();  // (every lane has read the count before the first of its digit raises it)
+  if (valid && before == 0) count[digit] = old + (uint32_t)__builtin_popcountll(same);
+  DFCCL_WAVE_LDS_SYNC();
+  return old + (uint32_t)__builtin_popcountll(before);
+}
+__device__ __forceinline__ uint32_t waveScan(uint32_t v, int lane) {  // inclusive
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t from = __shfl(v, (lane - d) & 63);
+    if (lane >= d) v += from;
+  }
+  return v;
+}
+
+// ---- a few thousand tokens: sorted by one workgroup in LDS, one launch instead of two per digit
+constexpr int kSmallThreads = 1024;
+constexpr int kSmallWaves = kSmallThreads / 64;
+constexpr int kSmallStrips = 4;
+constexpr uint32_t kSmallMax = kSmallThreads * kSmallStrips;
+constexpr int kSmallDigitBits = 8;
+constexpr int kSmallBins = 1 << kSmallDigitBits;
+
+__global__ __launch_bounds__(kSmallThreads) void sortSmallKernel(GradArgs a, int keyBits, Clear c) {
+  struct Shared {
+    uint32_t key[kSmallMax], pay[kSmallMax];
+    uint32_t count[kSmallWaves][kSmallBins];
+    uint32_t waveTotal[kSmallBins / 64];
+  };
+  DFCCL_WG_SHARED(Shared, sh);
+  if (blockIdx.x >= c.firstBlock) {
+    clearShare(c, kSmallWaves);
+    return;
+  }
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = waveInBlock();
+  const uint32_t start = (uint32_t)wave * (64 * kSmallStrips);
+  uint32_t key[kSmallStrips], pay[kSmallStrips], rank[kSmallStrips];
+#pragma unroll
+  for (int k = 0; k < kSmallStrips; k++) {
+    const uint32_t pos = start + k * 64 + lane;
+    key[k] = pay[k] = 0;
+    if (pos < a.n) keyOfToken(a, pos, key[k], pay[k]);
+  }
+  const int passes = (keyBits + kSmallDigitBits - 1) / kSmallDigitBits, bits = (keyBits + passes - 1) / passes;
+  for (int pass = 0; pass < passes; pass++) {
+    const int shift = pass * bits;
+    const uint32_t mask = (1u << bits) - 1;
+    for (int i = tid; i < kSmallWaves * kSmallBins; i += kSmallThreads) sh.count[i / kSmallBins][i % kSmallBins] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kSmallStrips; k++)
+      if (start + k * 64 < a.n)
+        rank[k] = rankInWave(sh.count[wave], (key[k] >> shift) & mask, bits, start + k * 64 + lane < a.n, lane);
+    __syncthreads();
+    // a digit's keys begin behind all keys of smaller digits, a wave's behind the same digit's of the waves before
+    uint32_t mine = 0, sum = 0;
+    if (tid < kSmallBins) {
+#pragma unroll
+      for (int w = 0; w < kSmallWaves; w++) mine += sh.count[w][tid];
+      sum = waveScan(mine, lane);
+      if (lane == 63) sh.waveTotal[wave] = sum;
+    }
+    __syncthreads();
+    if (tid < kSmallBins) {
+      uint32_t at = sum - mine;
+      for (int w = 0; w < wave; w++) at += sh.waveTotal[w];
+#pragma unroll
+      for (int w = 0; w < kSmallWaves; w++) {
+        const uint32_t n = sh.count[w][tid];
+        sh.count[w][tid] = at;
+        at += n;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kSmallStrips; k++)
+      if (start + k * 64 + lane < a.n) {
+        const uint32_t to = sh.count[wave][(key[k] >> shift) & mask] + rank[k];
+        sh.key[to] = key[k];
+        sh.pay[to] = pay[k];
+      }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kSmallStrips; k++) {
+      const uint32_t pos = start + k * 64 + lane;
+      if (pos < a.n) {
+        key[k] = sh.key[pos];
+        pay[k] = sh.pay[pos];
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kSmallStrips; k++) {
+    const uint32_t pos = start + k * 64 + lane;
+    if (pos < a.n) {
+      a.keys[0][pos] = key[k];
+      a.pays[0][pos] = pay[k];
+    }
+  }
+}
+
+// ---- more tokens: tiles, a count and a scatter per digit
 constexpr int kSortThreads = 256;
 constexpr int kSortWaves = kSortThreads / 64;
-// positions of a tile: short enough that a few thousand tokens spread over several workgroups, long enough that
+// strips of a tile: few enough that some ten thousand tokens spread over several workgroups, many enough that
 // the sum over the tiles' histograms, which every tile makes for itself, stays short
 constexpr int kShortStrips = 4, kLongStrips = 16;
 
-// Digit counts of every tile; the first pass also clears the rows' index with the workgroups behind the tiles.
 template <int S, bool FIRST>
-__global__ __launch_bounds__(kSortThreads) void sortCountKernel(GradArgs a, SortPass p) {
+__global__ __launch_bounds__(kSortThreads) void sortCountKernel(GradArgs a, SortPass p, Clear c) {
   struct Shared {
     uint32_t count[kMaxBins];
   };
   DFCCL_WG_SHARED(Shared, sh);
-  const int tid = (int)threadIdx.x, tile = (int)blockIdx.x, bins = 1 << p.bits;
-  if (FIRST && tile >= p.tiles) {
-    for (uint64_t i = (uint64_t)(tile - p.tiles) * kSortThreads + tid; i < a.rows;
-         i += (uint64_t)(gridDim.x - p.tiles) * kSortThreads)
-      a.rowBegin[i] = -1;
+  if (blockIdx.x >= c.firstBlock) {
+    clearShare(c, kSortWaves);
     return;
   }
+  const int tid = (int)threadIdx.x, tile = (int)blockIdx.x, bins = 1 << p.bits;
   for (int i = tid; i < bins; i += kSortThreads) sh.count[i] = 0;
   __syncthreads();
 #pragma unroll
@@ -205,10 +350,10 @@ __global__ __launch_bounds__(kSortThreads) void sortCountKernel(GradArgs a, Sort
   for (int i = tid; i < bins; i += kSortThreads) a.hist[(size_t)tile * bins + i] = sh.count[i];
 }
 
-// Stable scatter of a tile. A lane's rank among the tile's keys of the same digit: the equal digits of the waves
-// before, of this wave's strips before, and of the lanes before it in its strip (found with a ballot per bit).
+// Stable scatter of a tile: a key goes behind all keys of smaller digits, its digit's keys in the tiles before, in
+// the waves before, in the wave's strips before, and in the lanes before.
 template <int S, bool FIRST>
-__global__ __launch_bounds__(kSortThreads) void sortScatterKernel(GradArgs a, SortPass p) {
+__global__ __launch_bounds__(kSortThreads) void sortScatterKernel(GradArgs a, SortPass p, Clear c) {
   struct Shared {
     uint32_t count[kSortWaves][kMaxBins];
     uint32_t base[kMaxBins];
@@ -216,9 +361,11 @@ __global__ __launch_bounds__(kSortThreads) void sortScatterKernel(GradArgs a, So
     uint32_t waveTotal[kSortWaves];
   };
   DFCCL_WG_SHARED(Shared, sh);
+  if (blockIdx.x >= c.firstBlock) {
+    clearShare(c, kSortWaves);
+    return;
+  }
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = waveInBlock(), tile = (int)blockIdx.x, bins = 1 << p.bits;
-  for (int i = tid; i < kSortWaves * kMaxBins; i += kSortThreads) sh.count[i / kMaxBins][i % kMaxBins] = 0;
-  __syncthreads();
   uint32_t key[S], pay[S], rank[S];
   const uint64_t start = (uint64_t)tile * (kSortThreads * S) + (uint64_t)wave * (64 * S) + lane;
 #pragma unroll
@@ -233,46 +380,30 @@ __global__ __launch_bounds__(kSortThreads) void sortScatterKernel(GradArgs a, So
       }
     }
   }
-#pragma unroll
-  for (int k = 0; k < S; k++) {
-    const bool valid = start + k * 64 < a.n;
-    const uint32_t d = (key[k] >> p.shift) & (uint32_t)(bins - 1);
-    uint64_t same = __ballot(valid);
-    for (int b = 0; b < p.bits; b++) {
-      const bool one = (d >> b) & 1u;
-      const uint64_t ones = __ballot(one);
-      same &= one ? ones : ~ones;
-    }
-    const uint64_t before = same & ((1ull << lane) - 1);
-    const uint32_t old = sh.count[wave][d];
-    DFCCL_WAVE_LDS_SYNC();  // (every lane has read the count before the first of its digit raises it)
-    if (valid && before == 0) sh.count[wave][d] = old + (uint32_t)__builtin_popcountll(same);
-    DFCCL_WAVE_LDS_SYNC();
-    rank[k] = old + (uint32_t)__builtin_popcountll(before);
-  }
-  // where the tile's keys of each digit begin: all keys of smaller digits, then this digit's in the tiles before
   for (int i = tid; i < kMaxBins; i += kSortThreads) {
     uint32_t before = 0, total = 0;
-    if (i < bins)
+    if (i < bins) {
+#pragma unroll 8
       for (int t = 0; t < p.tiles; t++) {
         const uint32_t h = a.hist[(size_t)t * bins + i];
         before += t < tile ? h : 0;
         total += h;
       }
+    }
     sh.base[i] = before;
     sh.total[i] = total;
+#pragma unroll
+    for (int w = 0; w < kSortWaves; w++) sh.count[w][i] = 0;
   }
   __syncthreads();
+#pragma unroll
+  for (int k = 0; k < S; k++)
+    rank[k] = rankInWave(sh.count[wave], (key[k] >> p.shift) & (uint32_t)(bins - 1), p.bits, start + k * 64 < a.n, lane);
   constexpr int per = kMaxBins / kSortThreads;
   uint32_t mine = 0;
 #pragma unroll
   for (int i = 0; i < per; i++) mine += sh.total[tid * per + i];
-  uint32_t sum = mine;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t from = __shfl(sum, (lane - d) & 63);
-    if (lane >= d) sum += from;
-  }
+  const uint32_t sum = waveScan(mine, lane);
   if (lane == 63) sh.waveTotal[wave] = sum;
   __syncthreads();
   uint32_t at = sum - mine;
@@ -284,9 +415,9 @@ __global__ __launch_bounds__(kSortThreads) void sortScatterKernel(GradArgs a, So
     at += sh.total[bin];
 #pragma unroll
     for (int w = 0; w < kSortWaves; w++) {  // the waves' counts become where the waves' keys begin
-      const uint32_t c = sh.count[w][bin];
+      const uint32_t n = sh.count[w][bin];
       sh.count[w][bin] = next;
-      next += c;
+      next += n;
     }
   }
   __syncthreads();
@@ -299,40 +430,45 @@ __global__ __launch_bounds__(kSortThreads) void sortScatterKernel(GradArgs a, So
     }
 }
 
-// acc += the gradients of sorted positions [begin, end), this lane's eight columns, in order; eight loads in flight
+// ---- sums
+
+// acc += the gradients of `count` tokens (at most 64) whose payloads lanes from .. from + count - 1 hold, this lane's
+// eight columns, in order. The payloads come by lane, so the loads depend on nothing but each other's registers:
+// kAhead of them are in flight.
 template <int GT>
-__device__ __forceinline__ void addTokens(const GradArgs& a, const uint32_t* pays, uint32_t begin, uint32_t end,
-                                          uint32_t col, float (&acc)[kVec]) {
-  constexpr int kAhead = 8;
-  const bool full = col + kVec <= a.width;
+__device__ __forceinline__ void addTokens(const GradArgs& a, uint32_t pays, int from, int count, uint32_t col,
+                                          float (&acc)[kVec]) {
+  constexpr int kAhead = GT == kF32 ? 8 : 16;
   const int left = (int)a.width - (int)col;
-  for (uint32_t p = begin; p < end; p += kAhead) {
+  for (int p = 0; p < count; p += kAhead) {
     Raw8<GT> raw[kAhead];
-    if (full) {
 #pragma unroll
-      for (int i = 0; i < kAhead; i++)
-        if (p + i < end) {
-          const uint32_t pay = uniform(pays[p + i]);
-          raw[i] = loadRaw8<GT>(a.grads[pay >> kSrcShift] + (size_t)(pay & kTokenMask) * a.gradStride +
-                                (size_t)col * typeSize(GT));
+    for (int i = 0; i < kAhead; i++)
+      if (p + i < count) {
+        const uint32_t pay = (uint32_t)__builtin_amdgcn_readlane((int)pays, from + p + i);
+        const char* row = a.grads[pay >> kSrcShift] + (size_t)(pay & kTokenMask) * a.gradStride;
+        if (left >= kVec) {
+          raw[i] = loadRaw8<GT>(row + (size_t)col * typeSize(GT));
+        } else if (left > 0) {  // (the last, shorter vector of a row, put together from elements)
+          raw[i] = Raw8<GT>{};
+#pragma unroll
+          for (int j = 0; j < kVec - 1; j++)
+            if (j < left) {
+              const uint32_t e = (uint32_t)loadElem<typeSize(GT)>(row + (size_t)col * typeSize(GT), j);
+              if constexpr (GT == kF32) raw[i].w[j / 4][j % 4] = e;
+              else raw[i].w[0][j / 2] |= e << (16 * (j % 2));
+            }
         }
+      }
+    if (left > 0) {
 #pragma unroll
       for (int i = 0; i < kAhead; i++)
-        if (p + i < end) {
+        if (p + i < count) {
           float f[kVec];
           widen8<GT>(raw[i], f);
 #pragma unroll
           for (int j = 0; j < kVec; j++) acc[j] += f[j];
         }
-    } else if (left > 0) {
-      for (int i = 0; i < kAhead && p + i < end; i++) {
-        const uint32_t pay = uniform(pays[p + i]);
-        float f[kVec];
-        loadTail<GT>(a.grads[pay >> kSrcShift] + (size_t)(pay & kTokenMask) * a.gradStride + (size_t)col * typeSize(GT),
-                     left, f);
-#pragma unroll
-        for (int j = 0; j < kVec; j++) acc[j] += f[j];
-      }
     }
   }
 }
@@ -340,7 +476,7 @@ __device__ __forceinline__ void addTokens(const GradArgs& a, const uint32_t* pay
 __device__ __forceinline__ void addSums(const float* sums, uint32_t widthPad, uint32_t begin, uint32_t end, uint32_t col,
                                         float (&acc)[kVec]) {
   if (col >= widthPad) return;
-  constexpr int kAhead = 4;
+  constexpr int kAhead = 8;
   for (uint32_t c = begin; c < end; c += kAhead) {
     Raw8<kF32> raw[kAhead];
 #pragma unroll
@@ -357,30 +493,25 @@ __device__ __forceinline__ void addSums(const float* sums, uint32_t widthPad, ui
   }
 }
 
-// One wave per (chunk, piece): the chunk's sum if all of it belongs to one row; the first piece's waves also note
-// where rows begin and end.
+// One wave per (chunk, piece): the chunk's sum if all of it belongs to one row.
 template <int GT>
-__global__ __launch_bounds__(kRowThreads) void chunkKernel(GradArgs a, int sorted) {
+__global__ __launch_bounds__(kRowThreads) void chunkKernel(GradArgs a, int sorted, Clear c) {
+  if (blockIdx.x >= c.firstBlock) {
+    clearShare(c, kRowWaves);
+    return;
+  }
   const int lane = (int)(threadIdx.x & 63);
   const uint32_t* keys = a.keys[sorted];
-  const uint32_t chunks = (a.n + kChunk - 1) / kChunk;
-  const uint64_t items = (uint64_t)chunks * a.pieces;
+  const uint64_t items = (uint64_t)(a.n / kChunk) * a.pieces;
   for (uint64_t item = (uint64_t)blockIdx.x * kRowWaves + waveInBlock(); item < items;
-       item += (uint64_t)gridDim.x * kRowWaves) {
+       item += (uint64_t)c.firstBlock * kRowWaves) {
     const uint32_t chunk = (uint32_t)(item / a.pieces), piece = (uint32_t)(item % a.pieces), begin = chunk * kChunk;
-    if (piece == 0 && lane < kChunk && begin + lane < a.n) {
-      const uint32_t pos = begin + lane, key = keys[pos];
-      if (key < a.rows) {
-        if (pos == 0 || keys[pos - 1] != key) a.rowBegin[key] = (int32_t)pos;
-        if (pos + 1 == a.n || keys[pos + 1] != key) a.rowEnd[key] = pos + 1;
-      }
-    }
-    if (a.n - begin < kChunk) continue;
-    const uint32_t key = uniform(keys[begin]);
-    if (key >= a.rows || uniform(keys[begin + kChunk - 1]) != key) continue;
+    const uint32_t first = keys[begin], last = keys[begin + kChunk - 1], pays = a.pays[sorted][begin + (lane & (kChunk - 1))];
+    const uint32_t key = uniform(first);
+    if (key >= a.rows || uniform(last) != key) continue;
     const uint32_t col = piece * kPieceElems + lane * kVec;
     float acc[kVec] = {};
-    addTokens<GT>(a, a.pays[sorted], begin, begin + kChunk, col, acc);
+    addTokens<GT>(a, pays, 0, kChunk, col, acc);
     if (col < a.widthPad) store8<kF32>((char*)(a.chunkSums + (size_t)chunk * a.widthPad + col), acc);
   }
 }
@@ -388,13 +519,13 @@ __global__ __launch_bounds__(kRowThreads) void chunkKernel(GradArgs a, int sorte
 __global__ __launch_bounds__(kRowThreads) void superKernel(GradArgs a, int sorted) {
   const int lane = (int)(threadIdx.x & 63);
   const uint32_t* keys = a.keys[sorted];
-  const uint32_t supers = a.n / (kChunk * kChunk);
-  const uint64_t items = (uint64_t)supers * a.pieces;
+  const uint64_t items = (uint64_t)(a.n / (kChunk * kChunk)) * a.pieces;
   for (uint64_t item = (uint64_t)blockIdx.x * kRowWaves + waveInBlock(); item < items;
        item += (uint64_t)gridDim.x * kRowWaves) {
     const uint32_t super = (uint32_t)(item / a.pieces), piece = (uint32_t)(item % a.pieces);
-    const uint32_t begin = super * (kChunk * kChunk), key = uniform(keys[begin]);
-    if (key >= a.rows || uniform(keys[begin + kChunk * kChunk - 1]) != key) continue;
+    const uint32_t begin = super * (kChunk * kChunk), first = keys[begin], last = keys[begin + kChunk * kChunk - 1];
+    const uint32_t key = uniform(first);
+    if (key >= a.rows || uniform(last) != key) continue;
     const uint32_t col = piece * kPieceElems + lane * kVec;
     float acc[kVec] = {};
     addSums(a.chunkSums, a.widthPad, super * kChunk, (super + 1) * kChunk, col, acc);
@@ -402,35 +533,29 @@ __global__ __launch_bounds__(kRowThreads) void superKernel(GradArgs a, int sorte
   }
 }
 
-// acc = the sum of a row's run [begin, end)
-template <int GT>
-__device__ __forceinline__ void sumRun(const GradArgs& a, const uint32_t* pays, uint32_t begin, uint32_t end, uint32_t col,
-                                       float (&acc)[kVec]) {
-  const uint32_t c0 = (begin + kChunk - 1) / kChunk, c1 = end / kChunk;
-  if (c0 >= c1) {
-    addTokens<GT>(a, pays, begin, end, col, acc);
-    return;
+// The end of a run that is known to reach `lo`: the keys are sorted, so 64 lanes look at 64 places between lo and hi
+// and the search goes on between two of them.
+__device__ __forceinline__ uint32_t endOfRun(const uint32_t* keys, uint32_t key, uint32_t lo, uint32_t hi, int lane) {
+  while (lo < hi) {
+    const uint32_t step = (hi - lo + 63) / 64;
+    const uint64_t at = (uint64_t)lo + (uint64_t)lane * step;
+    const int in = __builtin_popcountll(__ballot(at < hi && keys[at < hi ? at : lo] == key));
+    if (in == 0) break;  // (the run ends at lo)
+    const uint64_t next = (uint64_t)lo + (uint64_t)in * step;
+    lo += (uint32_t)(in - 1) * step + 1;
+    if (next < hi) hi = (uint32_t)next;
   }
-  addTokens<GT>(a, pays, begin, c0 * kChunk, col, acc);
-  const uint32_t s0 = (c0 + kChunk - 1) / kChunk, s1 = c1 / kChunk;
-  if (s0 >= s1) {
-    addSums(a.chunkSums, a.widthPad, c0, c1, col, acc);
-  } else {
-    addSums(a.chunkSums, a.widthPad, c0, s0 * kChunk, col, acc);
-    addSums(a.superSums, a.widthPad, s0, s1, col, acc);
-    addSums(a.chunkSums, a.widthPad, s1 * kChunk, c1, col, acc);
-  }
-  addTokens<GT>(a, pays, c1 * kChunk, end, col, acc);
+  return lo;
 }
 
 template <int TT>
-__device__ __forceinline__ void writeRow(const GradArgs& a, uint32_t row, uint32_t col, bool accumulate, float (&acc)[kVec]) {
+__device__ __forceinline__ void writeRow(const GradArgs& a, uint32_t row, uint32_t col, float (&acc)[kVec]) {
   char* to = a.table + (size_t)row * a.tableStride + (size_t)col * typeSize(TT);
   const int left = (int)a.width - (int)col;
 #pragma unroll
   for (int j = 0; j < kVec; j++) acc[j] *= a.scale;
   if (left >= kVec) {
-    if (accumulate) {
+    if (a.accumulate) {
       float old[kVec];
       widen8<TT>(loadRaw8<TT>(to), old);
 #pragma unroll
@@ -438,7 +563,7 @@ __device__ __forceinline__ void writeRow(const GradArgs& a, uint32_t row, uint32
     }
     store8<TT>(to, acc);
   } else if (left > 0) {
-    if (accumulate) {
+    if (a.accumulate) {
       float old[kVec];
       loadTail<TT>(to, left, old);
 #pragma unroll
@@ -448,74 +573,90 @@ __device__ __forceinline__ void writeRow(const GradArgs& a, uint32_t row, uint32
   }
 }
 
-// Every row of the piece: kRowsPerWave rows' index is read at once.
-constexpr int kRowsPerWave = 4;
 template <int GT, int TT>
-__global__ __launch_bounds__(kRowThreads) void denseRowsKernel(GradArgs a, int sorted) {
+__global__ __launch_bounds__(kRowThreads) void rowsKernel(GradArgs a, int sorted) {
   const int lane = (int)(threadIdx.x & 63);
-  const uint64_t groups = ((uint64_t)a.rows + kRowsPerWave - 1) / kRowsPerWave, items = groups * a.pieces;
-  for (uint64_t item = (uint64_t)blockIdx.x * kRowWaves + waveInBlock(); item < items;
-       item += (uint64_t)gridDim.x * kRowWaves) {
-    const uint64_t row0 = item / a.pieces * kRowsPerWave;
-    const uint32_t col = (uint32_t)(item % a.pieces) * kPieceElems + (uint32_t)lane * kVec;
-    int32_t begin[kRowsPerWave];
-#pragma unroll
-    for (int i = 0; i < kRowsPerWave; i++) begin[i] = row0 + i < a.rows ? uniform(a.rowBegin[row0 + i]) : -1;
-#pragma unroll
-    for (int i = 0; i < kRowsPerWave; i++) {
-      if (row0 + i >= a.rows) break;
-      float acc[kVec] = {};
-      if (begin[i] >= 0) sumRun<GT>(a, a.pays[sorted], (uint32_t)begin[i], uniform(a.rowEnd[row0 + i]), col, acc);
-      writeRow<TT>(a, (uint32_t)(row0 + i), col, false, acc);
-    }
-  }
-}
-// The rows that tokens name: a wave per (position, piece) that goes on where its position begins a run.
-template <int GT, int TT>
-__global__ __launch_bounds__(kRowThreads) void namedRowsKernel(GradArgs a, int sorted) {
-  const int lane = (int)(threadIdx.x & 63);
-  const uint32_t* keys = a.keys[sorted];
+  const uint32_t *keys = a.keys[sorted], *pays = a.pays[sorted];
   const uint64_t items = (uint64_t)a.n * a.pieces;
   for (uint64_t item = (uint64_t)blockIdx.x * kRowWaves + waveInBlock(); item < items;
        item += (uint64_t)gridDim.x * kRowWaves) {
-    const uint32_t pos = (uint32_t)(item / a.pieces), key = uniform(keys[pos]);
-    if (key >= a.rows || (pos > 0 && uniform(keys[pos - 1]) == key)) continue;
+    const uint32_t pos = (uint32_t)(item / a.pieces);
+    // the keys from the one before on, and the payloads from this one on, a lane each: whether a run begins here,
+    // where it ends and whom it sums is known after one load
+    const uint64_t at = (uint64_t)pos + (uint32_t)lane;
+    const uint32_t window = at >= 1 && at - 1 < a.n ? keys[at - 1] : a.rows;
+    const uint32_t mine = at < a.n ? pays[at] : 0;
+    const uint32_t key = (uint32_t)__builtin_amdgcn_readlane((int)window, 1);
+    const uint32_t prev = (uint32_t)__builtin_amdgcn_readlane((int)window, 0);
+    if (key >= a.rows || prev == key) continue;
+    const uint64_t same = __ballot(window == key) >> 1;  // bit i: position pos + i
+    uint32_t end = pos + (uint32_t)__builtin_ctzll(~same);
+    if (end - pos == 63) end = endOfRun(keys, key, end, a.n, lane);
     const uint32_t col = (uint32_t)(item % a.pieces) * kPieceElems + (uint32_t)lane * kVec;
+    const uint32_t c0 = (pos + kChunk - 1) / kChunk, c1 = end / kChunk;
     float acc[kVec] = {};
-    sumRun<GT>(a, a.pays[sorted], pos, uniform(a.rowEnd[key]), col, acc);
-    writeRow<TT>(a, key, col, true, acc);
+    if (!a.chunked || c0 >= c1) {  // (fewer than 64 tokens either way)
+      addTokens<GT>(a, mine, 0, (int)(end - pos), col, acc);
+    } else {
+      const uint64_t behind = (uint64_t)c1 * kChunk + (uint32_t)lane;
+      const uint32_t rest = behind < end ? pays[behind] : 0;
+      addTokens<GT>(a, mine, 0, (int)(c0 * kChunk - pos), col, acc);
+      const uint32_t s0 = (c0 + kChunk - 1) / kChunk, s1 = c1 / kChunk;
+      if (!a.supered || s0 >= s1) {
+        addSums(a.chunkSums, a.widthPad, c0, c1, col, acc);
+      } else {
+        addSums(a.chunkSums, a.widthPad, c0, s0 * kChunk, col, acc);
+        addSums(a.superSums, a.widthPad, s0, s1, col, acc);
+        addSums(a.chunkSums, a.widthPad, s1 * kChunk, c1, col, acc);
+      }
+      addTokens<GT>(a, rest, 0, (int)(end - c1 * kChunk), col, acc);
+    }
+    writeRow<TT>(a, key, col, acc);
   }
 }
 
-typedef void (*GradKernel)(GradArgs, int);
-static GradKernel pickChunk(int gt) {
+typedef void (*SortKernel)(GradArgs, SortPass, Clear);
+template <int S, bool FIRST>
+static SortKernel pickSortS(bool scatter) {
+  return scatter ? sortScatterKernel<S, FIRST> : sortCountKernel<S, FIRST>;
+}
+static SortKernel pickSort(bool scatter, bool longTiles, bool first) {
+  if (longTiles) return first ? pickSortS<kLongStrips, true>(scatter) : pickSortS<kLongStrips, false>(scatter);
+  return first ? pickSortS<kShortStrips, true>(scatter) : pickSortS<kShortStrips, false>(scatter);
+}
+typedef void (*ChunkKernel)(GradArgs, int, Clear);
+typedef void (*RowsKernel)(GradArgs, int);
+static ChunkKernel pickChunk(int gt) {
   return gt == kF32 ? chunkKernel<kF32> : gt == kF16 ? chunkKernel<kF16> : chunkKernel<kBF16>;
 }
 template <int GT>
-static GradKernel pickRowsT(int tt, bool accumulate) {
-  if (accumulate)
-    return tt == kF32 ? namedRowsKernel<GT, kF32> : tt == kF16 ? namedRowsKernel<GT, kF16> : namedRowsKernel<GT, kBF16>;
-  return tt == kF32 ? denseRowsKernel<GT, kF32> : tt == kF16 ? denseRowsKernel<GT, kF16> : denseRowsKernel<GT, kBF16>;
+static RowsKernel pickRowsT(int tt) {
+  return tt == kF32 ? rowsKernel<GT, kF32> : tt == kF16 ? rowsKernel<GT, kF16> : rowsKernel<GT, kBF16>;
 }
-static GradKernel pickRows(int gt, int tt, bool accumulate) {
-  return gt == kF32 ? pickRowsT<kF32>(tt, accumulate) : gt == kF16 ? pickRowsT<kF16>(tt, accumulate) : pickRowsT<kBF16>(tt, accumulate);
+static RowsKernel pickRows(int gt, int tt) {
+  return gt == kF32 ? pickRowsT<kF32>(tt) : gt == kF16 ? pickRowsT<kF16>(tt) : pickRowsT<kBF16>(tt);
 }
 
-// Plan of a gradient call from its sizes: digits, tiles and where the workspace's parts begin.
+// Plan of a gradient call from its sizes: how it is sorted and where the workspace's parts begin.
 struct GradPlan {
-  int passes, digitBits, tiles;
-  bool longTiles;
-  size_t keys[2], pays[2], hist, rowBegin, rowEnd, chunkSums, superSums, bytes;
+  bool small, longTiles, chunked, supered;
+  int keyBits, passes, digitBits, tiles;
+  size_t keys[2], pays[2], hist, chunkSums, superSums, bytes;
 };
 static GradPlan planGrad(uint64_t n, size_t rows, size_t width) {
   GradPlan p{};
-  int bits = 1;
-  while (bits < 32 && ((uint64_t)rows >> bits) != 0) bits++;  // keys are 0 .. rows
-  p.passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
-  p.digitBits = (bits + p.passes - 1) / p.passes;
+  p.keyBits = 1;
+  while (p.keyBits < 32 && ((uint64_t)rows >> p.keyBits) != 0) p.keyBits++;  // keys are 0 .. rows
+  p.small = n <= kSmallMax;
+  p.passes = (p.keyBits + kMaxDigitBits - 1) / kMaxDigitBits;
+  p.digitBits = (p.keyBits + p.passes - 1) / p.passes;
   p.longTiles = n > 64u * 1024;
   const uint64_t tile = (uint64_t)kSortThreads * (p.longTiles ? kLongStrips : kShortStrips);
   p.tiles = (int)std::max<uint64_t>(1, (n + tile - 1) / tile);
+  // Runs of fewer than 64 tokens need no chunks. Chunks of chunks pay for their launch once a run may have several
+  // hundred chunks.
+  p.chunked = n >= 64;
+  p.supered = n >= 256 * kChunk;
   size_t at = 0;
   auto take = [&at](size_t bytes) {
     const size_t here = at;
@@ -523,16 +664,14 @@ static GradPlan planGrad(uint64_t n, size_t rows, size_t width) {
     return here;
   };
   const size_t widthPad = (width + kVec - 1) / kVec * kVec;
-  for (int i = 0; i < 2; i++) {
+  for (int i = 0; i < (p.small ? 1 : 2); i++) {
     p.keys[i] = take(n * 4);
     p.pays[i] = take(n * 4);
   }
-  p.hist = take(((size_t)p.tiles << p.digitBits) * 4);
-  p.rowBegin = take(rows * 4);
-  p.rowEnd = take(rows * 4);
-  p.chunkSums = take(n / kChunk * widthPad * 4);
-  p.superSums = take(n / (kChunk * kChunk) * widthPad * 4);
-  p.bytes = at;
+  if (!p.small) p.hist = take(((size_t)p.tiles << p.digitBits) * 4);
+  if (p.chunked) p.chunkSums = take(n / kChunk * widthPad * 4);
+  if (p.supered) p.superSums = take(n / (kChunk * kChunk) * widthPad * 4);
+  p.bytes = std::max<size_t>(at, 256);
   return p;
 }
 
@@ -637,43 +776,56 @@ DFCCL_API ncclResult_t dfcclEmbeddingGrad(const void* const* grads, const void* 
     a.keys[i] = (uint32_t*)(ws + p.keys[i]);
     a.pays[i] = (uint32_t*)(ws + p.pays[i]);
   }
+  a.accumulate = accumulate != 0;
+  a.chunked = p.chunked;
+  a.supered = p.supered;
   a.hist = (uint32_t*)(ws + p.hist);
-  a.rowBegin = (int32_t*)(ws + p.rowBegin);
-  a.rowEnd = (uint32_t*)(ws + p.rowEnd);
   a.chunkSums = (float*)(ws + p.chunkSums);
   a.superSums = (float*)(ws + p.superSums);
   a.widthPad = (uint32_t)((width + kVec - 1) / kVec * kVec);
 
+  // the table's clearing, in equal shares over the launches before the rows' sums
+  const int launches = (p.small ? 1 : 2 * p.passes) + (p.chunked ? 1 : 0);
+  Clear clear{};
+  uint64_t clearParts = 0;
+  if (!accumulate) {
+    const size_t rowBytes = width * typeSize((int)tableType);
+    const bool oneRow = a.tableStride == rowBytes;
+    clear.at = a.table;
+    clear.stride = a.tableStride;
+    clear.bytes = oneRow ? (uint64_t)rowBytes * rows : rowBytes;
+    clear.parts = (clear.bytes + kClearBytes - 1) / kClearBytes;
+    clearParts = clear.parts * (oneRow ? 1 : rows);
+  }
+  int launch = 0;
+  // the share of the next launch, whose own work takes `blocks` workgroups; returns the launch's grid
+  auto share = [&](unsigned blocks, unsigned waves) {
+    clear.begin = clearParts * launch / launches;
+    clear.end = clearParts * (launch + 1) / launches;
+    clear.firstBlock = blocks;
+    launch++;
+    const uint64_t want = (clear.end - clear.begin + waves - 1) / waves;
+    return blocks + (unsigned)std::min<uint64_t>(want, 256u * kClearWavesPerCu / waves);
+  };
   const hipStream_t st = (hipStream_t)stream;
   int from = 0;
-  for (int pass = 0; pass < p.passes; pass++, from ^= 1) {
-    SortPass s;
-    s.from = from;
-    s.shift = pass * p.digitBits;
-    s.bits = p.digitBits;
-    s.tiles = p.tiles;
-    const unsigned tiles = (unsigned)p.tiles;
-    if (pass == 0) {
-      const unsigned clear = accumulate ? 0u : (unsigned)std::min<size_t>((rows + 4095) / 4096, 1024);
-      DFCCL_LAUNCH_BLOCKS((p.longTiles ? sortCountKernel<kLongStrips, true> : sortCountKernel<kShortStrips, true>),
-                          tiles + clear, kSortThreads, st, a, s);
-      if (n == 0) break;
-      DFCCL_LAUNCH_BLOCKS((p.longTiles ? sortScatterKernel<kLongStrips, true> : sortScatterKernel<kShortStrips, true>), tiles,
-                          kSortThreads, st, a, s);
-    } else {
-      DFCCL_LAUNCH_BLOCKS((p.longTiles ? sortCountKernel<kLongStrips, false> : sortCountKernel<kShortStrips, false>), tiles,
-                          kSortThreads, st, a, s);
-      DFCCL_LAUNCH_BLOCKS((p.longTiles ? sortScatterKernel<kLongStrips, false> : sortScatterKernel<kShortStrips, false>), tiles,
-                          kSortThreads, st, a, s);
+  if (p.small) {
+    const unsigned grid = share(1, kSmallWaves);
+    DFCCL_LAUNCH_BLOCKS(sortSmallKernel, grid, kSmallThreads, st, a, p.keyBits, clear);
+  }
+  for (int pass = 0; !p.small && pass < p.passes; pass++, from ^= 1) {
+    const SortPass s{from, pass * p.digitBits, p.digitBits, p.tiles};
+    for (int scatter = 0; scatter < 2; scatter++) {
+      const unsigned grid = share((unsigned)p.tiles, kSortWaves);
+      DFCCL_LAUNCH_BLOCKS(pickSort(scatter != 0, p.longTiles, pass == 0), grid, kSortThreads, st, a, s, clear);
     }
   }
-  if (n > 0) {
-    const uint64_t chunks = (n + kChunk - 1) / kChunk;
-    DFCCL_LAUNCH_BLOCKS(pickChunk((int)gradType), gridFor(chunks * a.pieces), kRowThreads, st, a, from);
-    const uint64_t supers = n / (kChunk * kChunk);
-    if (supers > 0) DFCCL_LAUNCH_BLOCKS(superKernel, gridFor(supers * a.pieces), kRowThreads, st, a, from);
+  if (p.chunked) {
+    const unsigned grid = share(gridFor(n / kChunk * a.pieces), kRowWaves);
+    DFCCL_LAUNCH_BLOCKS(pickChunk((int)gradType), grid, kRowThreads, st, a, from, clear);
   }
-  const uint64_t waves = (accumulate ? n : ((uint64_t)rows + kRowsPerWave - 1) / kRowsPerWave) * a.pieces;
-  DFCCL_LAUNCH_BLOCKS(pickRows((int)gradType, (int)tableType, accumulate != 0), gridFor(waves), kRowThreads, st, a, from);
+  if (p.supered)
+    DFCCL_LAUNCH_BLOCKS(superKernel, gridFor(n / (kChunk * kChunk) * a.pieces), kRowThreads, st, a, from);
+  if (n > 0) DFCCL_LAUNCH_BLOCKS(pickRows((int)gradType, (int)tableType), gridFor(n * a.pieces), kRowThreads, st, a, from);
   return hipGetLastError() == hipSuccess ? ncclSuccess : ncclUnhandledCudaError;
 }

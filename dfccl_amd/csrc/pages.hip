@@ -26,6 +26,8 @@ constexpr int kScanThreads = DFCCL_SCAN_THREADS;
 constexpr int kScanWaves = kScanThreads / 64;
 constexpr int kScanPer = 4;  // counts a thread reads at once
 constexpr int kScanTile = kScanThreads * kScanPer;
+// Up to so many tiles one workgroup scans all pages; above, a workgroup per tile counts and another launch lists.
+constexpr int kOneScan = 4;
 
 // The bookkeeping as the kernels see it.
 struct Books {
@@ -43,7 +45,8 @@ struct PageScratch {
   int32_t* found;    // [pages] the lowest free pages (compact: the holes to fill), in order
   int32_t* movers;   // [pages] compact: the pages that move, in order
   int32_t* rank;     // [pages] compact: place among the movers
-  int32_t* counts;   // {pages found, pages that move}
+  int32_t* tiles;    // [tiles of pages] free (compact: live) pages of each
+  int32_t* counts;   // {pages found, pages that move, pages needed}
 };
 
 __device__ __forceinline__ int32_t pagesOf(int32_t tokens, int32_t pageTokens) {
@@ -81,42 +84,34 @@ __device__ __forceinline__ void loadCounts(const Books& b, int64_t first, int32_
   for (int i = 0; i < kScanPer; i++) c[i] = first + i < b.pages ? b.refcounts[first + i] : 1;
 }
 
-// The lowest `most` free pages, in order, into found; returns how many there are (at most `most`). One workgroup.
-__device__ __forceinline__ int32_t findFree(ScanShared& sh, const Books& b, int32_t* found, int64_t most) {
-  int64_t have = 0;
-  int which = 0;
-  for (int64_t at = 0; at < b.pages && have < most; at += kScanTile, which ^= 1) {
-    const int64_t first = at + (int64_t)threadIdx.x * kScanPer;
-    int32_t c[kScanPer];
-    loadCounts(b, first, c);
-    int32_t mine = 0, total;
+// One tile's free pages, in order, into found from place `have` on (as far as `most`); returns the tile's number.
+__device__ __forceinline__ int32_t listFree(ScanShared& sh, int which, const Books& b, int64_t tileAt, int64_t have, int64_t most,
+                                            int32_t* found) {
+  const int64_t first = tileAt + (int64_t)threadIdx.x * kScanPer;
+  int32_t c[kScanPer], mine = 0, total;
+  loadCounts(b, first, c);
 #pragma unroll
-    for (int i = 0; i < kScanPer; i++) mine += c[i] == 0;
-    int64_t to = have + blockScan(sh, which, mine, total);
+  for (int i = 0; i < kScanPer; i++) mine += c[i] == 0;
+  int64_t to = have + blockScan(sh, which, mine, total);
 #pragma unroll
-    for (int i = 0; i < kScanPer; i++)
-      if (c[i] == 0) {
-        if (to < most) found[to] = (int32_t)(first + i);
-        to++;
-      }
-    have += total;
-  }
-  return (int32_t)(have < most ? have : most);
+  for (int i = 0; i < kScanPer; i++)
+    if (c[i] == 0) {
+      if (to < most) found[to] = (int32_t)(first + i);
+      to++;
+    }
+  return total;
 }
 
-// ---- requests: which are valid, and which new pages each gets. One workgroup.
+// ---- requests: which are valid, and which of the new pages each gets
 struct Requests {
   const int32_t* a;  // extend: sequences; fork: parents
   const int32_t* b;  // extend: lengths;   fork: children
   int32_t n;
 };
-// extend: need = pages of the new length - pages of the old; fork: one page if the parent's last page is not full
+// extend: need = pages of the new length - pages of the old; fork: one page if the parent's last page is not full.
+// One workgroup; returns the pages that all of them need.
 template <bool FORK>
-__global__ __launch_bounds__(kScanThreads) void assignKernel(Books b, PageScratch s, Requests q) {
-  struct Shared {
-    ScanShared scan;
-  };
-  DFCCL_WG_SHARED(Shared, sh);
+__device__ __forceinline__ int32_t readRequests(ScanShared& sh, const Books& b, const PageScratch& s, const Requests& q) {
   const int tid = (int)threadIdx.x;
   const int64_t most = (int64_t)b.perSeq * b.pageTokens;
   // the first request that names a sequence (a fork: a child) has it; the others are refused
@@ -131,7 +126,7 @@ __global__ __launch_bounds__(kScanThreads) void assignKernel(Books b, PageScratc
       __hip_atomic_fetch_min(&s.owner[seq], i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
-  int64_t needed = 0;
+  int32_t needed = 0;  // (at most seqs * perSeq, which the host keeps below 2^31)
   int which = 0;
   for (int32_t at = 0; at < q.n; at += kScanThreads, which ^= 1) {
     const int32_t i = at + tid;
@@ -152,17 +147,75 @@ __global__ __launch_bounds__(kScanThreads) void assignKernel(Books b, PageScratc
       s.before[i] = before;
     }
     int32_t total;
-    const int32_t first = blockScan(sh.scan, which, need > 0 ? need : 0, total);
-    // (all needs together are at most seqs * perSeq, which the host keeps below 2^31)
-    if (i < q.n) s.request[i] = need < 0 ? -1 : (int32_t)needed + first;
+    const int32_t first = blockScan(sh, which, need > 0 ? need : 0, total);
+    if (i < q.n) s.request[i] = need < 0 ? -1 : needed + first;
     needed += total;
   }
   __syncthreads();
-  const int32_t have = findFree(sh.scan, b, s.found, needed);
-  if (tid == 0) {
-    s.counts[0] = have;
-    if (b.report != nullptr) b.report[0] = 0;  // the launch that follows counts the refusals
+  if (tid == 0 && b.report != nullptr) b.report[0] = 0;  // the launch that carries the requests out counts the refusals
+  return needed;
+}
+
+// A few tiles of pages: requests and free pages in one launch.
+template <bool FORK>
+__global__ __launch_bounds__(kScanThreads) void assignKernel(Books b, PageScratch s, Requests q) {
+  struct Shared {
+    ScanShared scan;
+  };
+  DFCCL_WG_SHARED(Shared, sh);
+  const int32_t needed = readRequests<FORK>(sh.scan, b, s, q);
+  int64_t have = 0;
+  int which = 0;
+  for (int64_t at = 0; at < b.pages && have < needed; at += kScanTile, which ^= 1)
+    have += listFree(sh.scan, which, b, at, have, needed, s.found);
+  if (threadIdx.x == 0) s.counts[0] = (int32_t)(have < needed ? have : needed);
+}
+
+// Many tiles, first launch: workgroup 0 reads the requests (a compaction has none), the others count a tile each.
+enum : int { kForExtend = 0, kForFork = 1, kForCompact = 2 };
+template <int FOR>
+__global__ __launch_bounds__(kScanThreads) void countTilesKernel(Books b, PageScratch s, Requests q) {
+  struct Shared {
+    ScanShared scan;
+  };
+  DFCCL_WG_SHARED(Shared, sh);
+  if (blockIdx.x == 0) {
+    if constexpr (FOR != kForCompact) {
+      const int32_t needed = readRequests<FOR == kForFork>(sh.scan, b, s, q);
+      if (threadIdx.x == 0) s.counts[2] = needed;
+    }
+    return;
   }
+  const int32_t tile = (int32_t)blockIdx.x - 1;
+  const int64_t first = (int64_t)tile * kScanTile + (int64_t)threadIdx.x * kScanPer;
+  int32_t c[kScanPer], mine = 0, total;
+  loadCounts(b, first, c);
+#pragma unroll
+  for (int i = 0; i < kScanPer; i++)
+    mine += FOR == kForCompact ? c[i] > 0 && first + i < b.pages : c[i] == 0;
+  (void)blockScan(sh.scan, 0, mine, total);
+  if (threadIdx.x == 0) s.tiles[tile] = total;
+}
+// The sum of the first n tiles' counts, by the workgroup.
+__device__ __forceinline__ int32_t sumTiles(ScanShared& sh, int which, const int32_t* tiles, int32_t n) {
+  int32_t mine = 0, total;
+  for (int32_t t = (int32_t)threadIdx.x; t < n; t += kScanThreads) mine += tiles[t];
+  (void)blockScan(sh, which, mine, total);
+  return total;
+}
+// Second launch: a workgroup per tile lists the tile's free pages behind those of the tiles before.
+__global__ __launch_bounds__(kScanThreads) void listFreeKernel(Books b, PageScratch s, int32_t tiles) {
+  struct Shared {
+    ScanShared scan;
+  };
+  DFCCL_WG_SHARED(Shared, sh);
+  const int32_t tile = (int32_t)blockIdx.x, needed = s.counts[2];
+  const int32_t have = sumTiles(sh.scan, 0, s.tiles, tile);
+  if (tile + 1 == tiles && threadIdx.x == 0) {
+    const int32_t all = have + s.tiles[tile];
+    s.counts[0] = all < needed ? all : needed;
+  }
+  if (have < needed) (void)listFree(sh.scan, 1, b, (int64_t)tile * kScanTile, have, needed, s.found);
 }
 
 __device__ __forceinline__ void refuse(const Books& b) {
@@ -248,16 +301,17 @@ __global__ __launch_bounds__(kMoveThreads) void copyKernel(PoolSet p, const int3
   }
 }
 
-// Fork, the tables: one workgroup per request. The child's whole pages are the parent's; a last page that is not full
-// is the child's own, its contents copied by forkMoveKernel (from the table rows, which this kernel's launch precedes).
-__global__ __launch_bounds__(kMoveThreads) void forkKernel(Books b, PageScratch s, Requests q) {
-  for (int32_t i = (int32_t)blockIdx.x; i < q.n; i += (int32_t)gridDim.x) {
-    const int32_t first = s.request[i];
-    const int32_t before = s.before[i];
+// Fork. The first q.n workgroups (of the first launch, if the pools take several) write the tables, one per request:
+// the child's whole pages are the parent's, a last page that is not full is the child's own. The others copy the
+// contents of those. Neither reads what the other writes: children were empty, and parents stay as they are.
+__global__ __launch_bounds__(kMoveThreads) void forkKernel(Books b, PageScratch s, Requests q, PoolSet p, uint32_t tableBlocks) {
+  if (blockIdx.x < tableBlocks) {
+    const int32_t i = (int32_t)blockIdx.x;
+    const int32_t first = s.request[i], before = s.before[i];
     const int32_t whole = before / b.pageTokens, need = before % b.pageTokens != 0;
     if (first < 0 || (need != 0 && first >= s.counts[0])) {
       if (threadIdx.x == 0) refuse(b);
-      continue;
+      return;
     }
     const int32_t parent = q.a[i], child = q.b[i];
     const int32_t* from = b.tables + (size_t)parent * b.perSeq;
@@ -275,14 +329,13 @@ __global__ __launch_bounds__(kMoveThreads) void forkKernel(Books b, PageScratch 
       }
       b.lengths[child] = before;
     }
+    return;
   }
-}
-__global__ __launch_bounds__(kMoveThreads) void forkMoveKernel(Books b, PageScratch s, Requests q, PoolSet p) {
   const int lane = (int)(threadIdx.x & 63);
   const uint32_t perPair = (uint32_t)p.npools * p.parts;
   const uint64_t items = (uint64_t)q.n * perPair;
-  for (uint64_t item = (uint64_t)blockIdx.x * kMoveWaves + waveInBlock(); item < items;
-       item += (uint64_t)gridDim.x * kMoveWaves) {
+  for (uint64_t item = (uint64_t)(blockIdx.x - tableBlocks) * kMoveWaves + waveInBlock(); item < items;
+       item += (uint64_t)(gridDim.x - tableBlocks) * kMoveWaves) {
     const uint32_t i = (uint32_t)(item / perPair);
     const int32_t first = uniform(s.request[i]), before = uniform(s.before[i]);
     if (first < 0 || before % b.pageTokens == 0 || first >= uniform(s.counts[0])) continue;
@@ -372,44 +425,96 @@ __global__ __launch_bounds__(kScanThreads) void compactPlanKernel(Books b, PageS
     }
   }
 }
-__global__ __launch_bounds__(kMoveThreads) void compactMoveKernel(Books b, PageScratch s, PoolSet p) {
-  const int lane = (int)(threadIdx.x & 63);
-  const uint32_t perPair = (uint32_t)p.npools * p.parts;
-  const uint64_t items = (uint64_t)uniform(s.counts[1]) * perPair;
-  for (uint64_t item = (uint64_t)blockIdx.x * kMoveWaves + waveInBlock(); item < items;
-       item += (uint64_t)gridDim.x * kMoveWaves) {
-    const uint32_t i = (uint32_t)(item / perPair);
-    moveItem(p, uniform(s.movers[i]), uniform(s.found[i]), (uint32_t)(item % perPair), lane);
+// The plan over many tiles, second launch: a workgroup per tile. With the live pages before a page known, a hole's
+// place is the number of free pages before it, and a mover's the number of live pages between L and it.
+__global__ __launch_bounds__(kScanThreads) void listMovesKernel(Books b, PageScratch s, int32_t tiles) {
+  struct Shared {
+    ScanShared scan;
+  };
+  DFCCL_WG_SHARED(Shared, sh);
+  const int32_t tile = (int32_t)blockIdx.x;
+  const int32_t live = sumTiles(sh.scan, 0, s.tiles, tiles), before = sumTiles(sh.scan, 1, s.tiles, tile);
+  __syncthreads();
+  const int32_t edge = live / kScanTile;  // the tile that L lies in, or the one behind the last
+  int32_t below = sumTiles(sh.scan, 0, s.tiles, edge);
+  const int64_t edgeAt = (int64_t)edge * kScanTile + (int64_t)threadIdx.x * kScanPer, first =
+      (int64_t)tile * kScanTile + (int64_t)threadIdx.x * kScanPer;
+  int32_t c[kScanPer], mine = 0, total;
+  loadCounts(b, edgeAt, c);
+#pragma unroll
+  for (int i = 0; i < kScanPer; i++) mine += edgeAt + i < live && c[i] > 0;
+  (void)blockScan(sh.scan, 1, mine, total);
+  below += total;  // live pages below L
+  __syncthreads();
+  mine = 0;
+  loadCounts(b, first, c);
+#pragma unroll
+  for (int i = 0; i < kScanPer; i++) mine += first + i < b.pages && c[i] > 0;
+  int32_t liveBefore = before + blockScan(sh.scan, 0, mine, total);
+#pragma unroll
+  for (int i = 0; i < kScanPer; i++)
+    if (first + i < b.pages) {
+      const int32_t page = (int32_t)(first + i);
+      if (c[i] <= 0) {
+        if (page < live) s.found[page - liveBefore] = page;
+      } else {
+        if (page >= live) {
+          s.rank[page] = liveBefore - below;
+          s.movers[liveBefore - below] = page;
+        }
+        liveBefore++;
+      }
+    }
+  if (tile == 0 && threadIdx.x == 0) {
+    s.counts[1] = live - below;
+    if (b.report != nullptr) {
+      b.report[1] = live - below;
+      b.report[2] = live;
+    }
   }
 }
-// Compact, the bookkeeping: table entries follow the moves, and the counts move with their pages.
-__global__ __launch_bounds__(kMoveThreads) void compactBooksKernel(Books b, PageScratch s) {
-  const int32_t moves = s.counts[1];
-  for (int32_t i = (int32_t)(blockIdx.x * kMoveThreads + threadIdx.x); i < moves; i += (int32_t)(gridDim.x * kMoveThreads)) {
-    const int32_t from = s.movers[i], to = s.found[i];
-    b.refcounts[to] = b.refcounts[from];
-    b.refcounts[from] = 0;
-  }
-  for (int32_t seq = (int32_t)blockIdx.x; seq < b.seqs; seq += (int32_t)gridDim.x) {
-    const int32_t length = b.lengths[seq];
-    if (length <= 0) continue;
-    int32_t used = pagesOf(length, b.pageTokens);
-    if (used > b.perSeq) used = b.perSeq;
-    int32_t* row = b.tables + (size_t)seq * b.perSeq;
-    for (int32_t k = (int32_t)threadIdx.x; k < used; k += kMoveThreads) {
-      const int32_t page = row[k];
-      if (page < 0 || page >= b.pages) continue;
-      const int32_t r = s.rank[page];  // (left over from anywhere for a page that does not move)
-      if (r >= 0 && r < moves && s.movers[r] == page) row[k] = s.found[r];
+
+// Compact, the moves: the first bookBlocks workgroups (of the first launch) let table entries and counts follow, the
+// others move the contents.
+__global__ __launch_bounds__(kMoveThreads) void compactKernel(Books b, PageScratch s, PoolSet p, uint32_t bookBlocks) {
+  const int32_t moves = uniform(s.counts[1]);
+  if (blockIdx.x < bookBlocks) {
+    for (int32_t i = (int32_t)(blockIdx.x * kMoveThreads + threadIdx.x); i < moves; i += (int32_t)(bookBlocks * kMoveThreads)) {
+      const int32_t from = s.movers[i], to = s.found[i];
+      b.refcounts[to] = b.refcounts[from];
+      b.refcounts[from] = 0;
     }
+    for (int32_t seq = (int32_t)blockIdx.x; seq < b.seqs; seq += (int32_t)bookBlocks) {
+      const int32_t length = b.lengths[seq];
+      if (length <= 0) continue;
+      int32_t used = pagesOf(length, b.pageTokens);
+      if (used > b.perSeq) used = b.perSeq;
+      int32_t* row = b.tables + (size_t)seq * b.perSeq;
+      for (int32_t k = (int32_t)threadIdx.x; k < used; k += kMoveThreads) {
+        const int32_t page = row[k];
+        if (page < 0 || page >= b.pages) continue;
+        const int32_t r = s.rank[page];  // (left over from anywhere for a page that does not move)
+        if (r >= 0 && r < moves && s.movers[r] == page) row[k] = s.found[r];
+      }
+    }
+    return;
+  }
+  const int lane = (int)(threadIdx.x & 63);
+  const uint32_t perPair = (uint32_t)p.npools * p.parts;
+  const uint64_t items = (uint64_t)moves * perPair;
+  for (uint64_t item = (uint64_t)(blockIdx.x - bookBlocks) * kMoveWaves + waveInBlock(); item < items;
+       item += (uint64_t)(gridDim.x - bookBlocks) * kMoveWaves) {
+    const uint32_t i = (uint32_t)(item / perPair);
+    moveItem(p, uniform(s.movers[i]), uniform(s.found[i]), (uint32_t)(item % perPair), lane);
   }
 }
 
 // ---- host
 
 struct PagePlan {
-  size_t owner, request, before, found, movers, rank, counts, bytes;
+  size_t owner, request, before, found, movers, rank, tiles, counts, bytes;
 };
+static int64_t tilesOf(int64_t pages) { return (pages + kScanTile - 1) / kScanTile; }
 static PagePlan planPages(int64_t pages, int64_t seqs) {
   PagePlan p{};
   size_t at = 0;
@@ -424,6 +529,7 @@ static PagePlan planPages(int64_t pages, int64_t seqs) {
   p.found = take(pages);
   p.movers = take(pages);
   p.rank = take(pages);
+  p.tiles = take(tilesOf(pages));
   p.counts = take(4);
   p.bytes = at;
   return p;
@@ -467,6 +573,7 @@ static PageScratch scratchOf(const dfcclPageCache* c) {
   s.found = (int32_t*)(ws + p.found);
   s.movers = (int32_t*)(ws + p.movers);
   s.rank = (int32_t*)(ws + p.rank);
+  s.tiles = (int32_t*)(ws + p.tiles);
   s.counts = (int32_t*)(ws + p.counts);
   return s;
 }
@@ -485,6 +592,16 @@ static PoolSet poolSet(const dfcclPageCache* to, const dfcclPageCache* from, int
 constexpr uint64_t kMaxMoveGrid = 1u << 22;
 static unsigned moveGrid(uint64_t items) {
   return (unsigned)std::max<uint64_t>(1, std::min<uint64_t>((items + kMoveWaves - 1) / kMoveWaves, kMaxMoveGrid));
+}
+template <int FOR>
+static void launchAssign(const Books& b, const PageScratch& s, const Requests& q, hipStream_t st) {
+  const int32_t tiles = (int32_t)tilesOf(b.pages);
+  if (tiles <= kOneScan) {
+    DFCCL_LAUNCH_BLOCKS(assignKernel<FOR == kForFork>, 1, kScanThreads, st, b, s, q);
+  } else {
+    DFCCL_LAUNCH_BLOCKS(countTilesKernel<FOR>, (unsigned)tiles + 1, kScanThreads, st, b, s, q);
+    DFCCL_LAUNCH_BLOCKS(listFreeKernel, (unsigned)tiles, kScanThreads, st, b, s, tiles);
+  }
 }
 static ncclResult_t launched() { return hipGetLastError() == hipSuccess ? ncclSuccess : ncclUnhandledCudaError; }
 // a page's parts over a launch's pools are counted in 32 bits
@@ -524,7 +641,7 @@ DFCCL_API ncclResult_t dfcclPagesExtend(const dfcclPageCache* c, const int32_t* 
   const hipStream_t st = (hipStream_t)stream;
   const PageScratch s = scratchOf(c);
   const Requests q{sequences, lengths, n};
-  DFCCL_LAUNCH_BLOCKS(assignKernel<false>, 1, kScanThreads, st, b, s, q);
+  launchAssign<kForExtend>(b, s, q, st);
   if (n > 0) DFCCL_LAUNCH_BLOCKS(extendKernel, (unsigned)n, kMoveThreads, st, b, s, q);
   return launched();
 }
@@ -537,13 +654,12 @@ DFCCL_API ncclResult_t dfcclPagesFork(const dfcclPageCache* c, const int32_t* pa
   const hipStream_t st = (hipStream_t)stream;
   const PageScratch s = scratchOf(c);
   const Requests q{parents, children, n};
-  DFCCL_LAUNCH_BLOCKS(assignKernel<true>, 1, kScanThreads, st, b, s, q);
-  if (n > 0) {
-    DFCCL_LAUNCH_BLOCKS(forkKernel, (unsigned)n, kMoveThreads, st, b, s, q);
-    for (int first = 0; first < c->npools; first += kMaxPools) {
-      const PoolSet p = poolSet(c, c, first);
-      DFCCL_LAUNCH_BLOCKS(forkMoveKernel, moveGrid((uint64_t)n * p.npools * p.parts), kMoveThreads, st, b, s, q, p);
-    }
+  launchAssign<kForFork>(b, s, q, st);
+  for (int first = 0; n > 0 && first < c->npools; first += kMaxPools) {
+    const PoolSet p = poolSet(c, c, first);
+    const unsigned tableBlocks = first == 0 ? (unsigned)n : 0u;
+    DFCCL_LAUNCH_BLOCKS(forkKernel, tableBlocks + moveGrid((uint64_t)n * p.npools * p.parts), kMoveThreads, st, b, s, q, p,
+                        tableBlocks);
   }
   return launched();
 }
@@ -560,13 +676,19 @@ DFCCL_API ncclResult_t dfcclPagesCompact(const dfcclPageCache* c, void* stream) 
   const Books b = booksOf(c);
   const PageScratch s = scratchOf(c);
   const hipStream_t st = (hipStream_t)stream;
-  DFCCL_LAUNCH_BLOCKS(compactPlanKernel, 1, kScanThreads, st, b, s);
+  const int32_t tiles = (int32_t)tilesOf(b.pages);
+  if (tiles <= kOneScan) {
+    DFCCL_LAUNCH_BLOCKS(compactPlanKernel, 1, kScanThreads, st, b, s);
+  } else {
+    DFCCL_LAUNCH_BLOCKS(countTilesKernel<kForCompact>, (unsigned)tiles + 1, kScanThreads, st, b, s, Requests{});
+    DFCCL_LAUNCH_BLOCKS(listMovesKernel, (unsigned)tiles, kScanThreads, st, b, s, tiles);
+  }
   for (int first = 0; first < c->npools; first += kMaxPools) {
     const PoolSet p = poolSet(c, c, first);
     // how many pages move is known on the GPU only: at most half of them
     const uint64_t most = (uint64_t)(c->pages / 2) * p.npools * p.parts;
-    DFCCL_LAUNCH_BLOCKS(compactMoveKernel, std::min(moveGrid(most), 2048u), kMoveThreads, st, b, s, p);
+    const unsigned bookBlocks = first == 0 ? (unsigned)std::min(c->sequences, 2048) : 0u;
+    DFCCL_LAUNCH_BLOCKS(compactKernel, bookBlocks + std::min(moveGrid(most), 2048u), kMoveThreads, st, b, s, p, bookBlocks);
   }
-  DFCCL_LAUNCH_BLOCKS(compactBooksKernel, (unsigned)std::min(c->sequences, 2048), kMoveThreads, st, b, s);
   return launched();
 }

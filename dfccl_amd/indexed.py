@@ -1,30 +1,37 @@
 """Rows of a table and pages of a cache that are named by an index on the GPU: the embedding lookup and its gradient,
 and the page operations of a cache, over the C ABI (dfcclEmbedding*, dfcclPages* in include/ofccl.h).  As everywhere
 in this layer, buffers are torch tensors on the GPU, calls are asynchronous on `stream` (default: torch's current
-stream) and the entry points check sizes; what is checked here is what a pointer no longer tells."""
+stream) and the entry points check sizes; what is checked here is what a pointer no longer tells.
+
+A call on a few rows or pages takes the GPU some three microseconds, so the checks avoid what costs as much on the
+host: no tensor is made, and torch is asked for nothing twice."""
 import ctypes
-import functools
 
 import torch
 
 from . import _lib, api
 
-_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+_FLOATS = frozenset((torch.float32, torch.float16, torch.bfloat16))
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the current stream's handle without an object
 
 
-def _stream_of(t, stream):
-    return ctypes.c_void_p((torch.cuda.current_stream(t.device) if stream is None else stream).cuda_stream)
+def _stream_of(device, stream):
+    if stream is not None:
+        return stream.cuda_stream
+    if device.type == "cuda" and _raw_stream is not None:
+        return _raw_stream(device.index)
+    return torch.cuda.current_stream(device).cuda_stream
 
 
-def _on_device_of(fn):
-    """Runs fn with the current device that of its `where` tensor, as a launch on that device's streams needs it."""
-    @functools.wraps(fn)
-    def wrapped(where, *args):
-        if where.is_cuda and where.device.index != torch.cuda.current_device():
-            with torch.cuda.device(where.device):
-                return fn(where, *args)
-        return fn(where, *args)
-    return wrapped
+def _call(device, fn, what, *args):
+    """Runs an entry point with `device` as the current one, as a launch on that device's streams needs it."""
+    if device.type == "cuda" and device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            code = fn(*args)
+    else:
+        code = fn(*args)
+    if code != 0:
+        api.check(code, what)
 
 
 def _rows_ptr(t, what):
@@ -40,35 +47,33 @@ def _rows_ptr(t, what):
     return api._dev_ptr(t[0]), t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _ids_ptr(ids):
-    if ids.dtype not in (torch.int32, torch.int64):
+def _ids_ptr(ids, device):
+    if ids.dtype is not torch.int64 and ids.dtype is not torch.int32:
         raise TypeError(f"ids: dtype {ids.dtype} is not int32 or int64")
+    _on(device, ids)
     return api._dev_ptr(ids)
 
 
-def _same_device(first, *others):
-    for t in others:
-        if t.device != first.device:
-            raise ValueError(f"tensors on {first.device} and {t.device}: one call works on one device")
-
-
-@_on_device_of
-def _call(where, fn, what, *args):
-    api.check(fn(*args), what)
+def _on(device, *tensors):
+    for t in tensors:
+        if t.device != device:
+            raise ValueError(f"tensors on {device} and {t.device}: one call works on one device")
 
 
 def embedding_lookup(table, ids, out, scale=1.0, first_row=0, stream=None):
     """out[t, :] = scale * table[ids[t] - first_row, :] (dfcclEmbeddingLookup), zeros for ids outside the table, which
     may be one rank's piece of the vocabulary.  ids may have any shape, out is [ids.numel(), width]; rows of `table`
     and `out` may be further apart than their width."""
-    _same_device(table, ids, out)
     table_ptr, table_stride = _rows_ptr(table, "table")
     out_ptr, out_stride = _rows_ptr(out, "out")
-    if out.shape[0] != ids.numel() or out.shape[1] != table.shape[1]:
-        raise ValueError(f"out has shape {tuple(out.shape)}, not {(ids.numel(), table.shape[1])}")
-    _call(table, _lib.load().dfcclEmbeddingLookup, "dfcclEmbeddingLookup", table_ptr, api.nccl_dtype(table),
-          table.shape[0], table_stride, first_row, _ids_ptr(ids), api.nccl_dtype(ids), ids.numel(), table.shape[1], scale,
-          out_ptr, api.nccl_dtype(out), out_stride, _stream_of(table, stream))
+    rows, width = table.shape
+    tokens, device = ids.numel(), table.device
+    if tuple(out.shape) != (tokens, width):
+        raise ValueError(f"out has shape {tuple(out.shape)}, not {(tokens, width)}")
+    _on(device, out)
+    _call(device, _lib.load().dfcclEmbeddingLookup, "dfcclEmbeddingLookup", table_ptr, api.DTYPE_OF[table.dtype], rows,
+          table_stride, first_row, _ids_ptr(ids, device), api.DTYPE_OF[ids.dtype], tokens, width, scale, out_ptr,
+          api.DTYPE_OF[out.dtype], out_stride, _stream_of(device, stream))
 
 
 def embedding_grad_workspace(tokens, rows, width):
@@ -86,39 +91,43 @@ def embedding_grad(grads, ids, table_grad, scale=1.0, first_row=0, padding_id=No
     padding_id are left out.  accumulate: add to the rows that tokens name instead of writing all rows.  workspace: a
     tensor of at least embedding_grad_workspace() bytes (default: one is allocated)."""
     if isinstance(grads, torch.Tensor):
-        grads, ids = [grads], [ids]
-    if len(grads) != len(ids) or not grads:
+        grads, ids = (grads,), (ids,)
+    n = len(grads)
+    if n != len(ids) or n == 0:
         raise ValueError("as many ids as gradients, and at least one of each")
-    _same_device(table_grad, *grads, *ids)
     table_ptr, table_stride = _rows_ptr(table_grad, "table_grad")
     rows, width = table_grad.shape
-    n = len(grads)
-    grad_ptrs, id_ptrs, tokens, strides = (ctypes.c_void_p * n)(), (ctypes.c_void_p * n)(), [], set()
-    for r, (g, i) in enumerate(zip(grads, ids)):
+    device, dtype, id_type = table_grad.device, grads[0].dtype, ids[0].dtype
+    grad_ptrs, id_ptrs, sizes = (ctypes.c_void_p * n)(), (ctypes.c_void_p * n)(), (ctypes.c_size_t * n)()
+    grad_stride = None
+    for r in range(n):
+        g, i = grads[r], ids[r]
         grad_ptrs[r], stride = _rows_ptr(g, "grads")
-        id_ptrs[r] = _ids_ptr(i)
-        if g.dtype != grads[0].dtype or i.dtype != ids[0].dtype:
+        id_ptrs[r] = _ids_ptr(i, device)
+        if g.dtype != dtype or i.dtype != id_type:
             raise ValueError("the sources must agree in dtype")
-        if g.shape[0] != i.numel() or g.shape[1] != width:
-            raise ValueError(f"grads[{r}] has shape {tuple(g.shape)}, not {(i.numel(), width)}")
-        tokens.append(g.shape[0])
-        if g.shape[0] > 1:
-            strides.add(stride)
-    if len(strides) > 1:
-        raise ValueError("the sources must agree in their row stride")
+        tokens = i.numel()
+        if tuple(g.shape) != (tokens, width):
+            raise ValueError(f"grads[{r}] has shape {tuple(g.shape)}, not {(tokens, width)}")
+        _on(device, g)
+        sizes[r] = tokens
+        if tokens > 1:
+            if grad_stride is not None and grad_stride != stride:
+                raise ValueError("the sources must agree in their row stride")
+            grad_stride = stride
     lib = _lib.load()
-    sizes = (ctypes.c_size_t * n)(*tokens)
-    need = ctypes.c_size_t()
-    api.check(lib.dfcclEmbeddingGradWorkspace(n, sizes, rows, width, ctypes.byref(need)), "dfcclEmbeddingGradWorkspace")
     if workspace is None:
-        workspace = torch.empty(need.value, dtype=torch.uint8, device=table_grad.device)
-        if stream is not None and table_grad.is_cuda:
+        need = ctypes.c_size_t()
+        api.check(lib.dfcclEmbeddingGradWorkspace(n, sizes, rows, width, ctypes.byref(need)), "dfcclEmbeddingGradWorkspace")
+        workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
+        if stream is not None and workspace.is_cuda:
             workspace.record_stream(stream)
-    _same_device(table_grad, workspace)
-    _call(table_grad, lib.dfcclEmbeddingGrad, "dfcclEmbeddingGrad", grad_ptrs, id_ptrs, sizes, n, api.nccl_dtype(grads[0]),
-          strides.pop() if strides else width, api.nccl_dtype(ids[0]), first_row, rows, width,
-          -1 if padding_id is None else padding_id, scale, int(accumulate), table_ptr, api.nccl_dtype(table_grad),
-          table_stride, api._dev_ptr(workspace), workspace.numel() * workspace.element_size(), _stream_of(table_grad, stream))
+    else:
+        _on(device, workspace)
+    _call(device, lib.dfcclEmbeddingGrad, "dfcclEmbeddingGrad", grad_ptrs, id_ptrs, sizes, n, api.DTYPE_OF[dtype],
+          width if grad_stride is None else grad_stride, api.DTYPE_OF[id_type], first_row, rows, width,
+          -1 if padding_id is None else padding_id, scale, int(accumulate), table_ptr, api.DTYPE_OF[table_grad.dtype],
+          table_stride, api._dev_ptr(workspace), workspace.numel() * workspace.element_size(), _stream_of(device, stream))
 
 
 class PageCache:
@@ -128,30 +137,32 @@ class PageCache:
     requests refused by the last extend or fork; report[1], report[2]: pages moved, pages live at the last compact."""
 
     def __init__(self, pools, page_tokens, refcounts, tables, lengths):
-        pages = pools[0].shape[0]
-        page_bytes = pools[0].numel() // max(1, pages) * pools[0].element_size()
+        pages, size = pools[0].shape[0], pools[0].numel() * pools[0].element_size()
+        device = refcounts.device
         for p in pools:
-            if p.shape[0] != pages or p.numel() * p.element_size() != pages * page_bytes:
+            if p.shape[0] != pages or p.numel() * p.element_size() != size:
                 raise ValueError("the pools must agree in pages and bytes per page")
         for t in (refcounts, tables, lengths):
             if t.dtype != torch.int32:
                 raise TypeError("the bookkeeping is held in int32 tensors")
         if refcounts.shape != (pages,) or tables.dim() != 2 or lengths.shape != (tables.shape[0],):
             raise ValueError("refcounts is [pages], tables [sequences, pages per sequence], lengths [sequences]")
-        _same_device(refcounts, tables, lengths, *pools)
-        self.lib = _lib.load()
+        _on(device, tables, lengths, *pools)
+        lib = _lib.load()
         need = ctypes.c_size_t()
-        api.check(self.lib.dfcclPageCacheWorkspace(pages, tables.shape[0], ctypes.byref(need)), "dfcclPageCacheWorkspace")
+        api.check(lib.dfcclPageCacheWorkspace(pages, tables.shape[0], ctypes.byref(need)), "dfcclPageCacheWorkspace")
         self.pools, self.page_tokens = pools, page_tokens
         self.refcounts, self.tables, self.lengths = refcounts, tables, lengths
-        self.report = torch.zeros(3, dtype=torch.int32, device=refcounts.device)
-        self._workspace = torch.empty(need.value, dtype=torch.uint8, device=refcounts.device)
+        self.report = torch.zeros(3, dtype=torch.int32, device=device)
+        self._device = device
+        self._workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
         self._pointers = (ctypes.c_void_p * len(pools))(*[api._dev_ptr(p).value for p in pools])
         self._struct = _lib.PageCacheStruct(
-            ctypes.sizeof(_lib.PageCacheStruct), self._pointers, page_bytes, len(pools), pages, page_tokens, tables.shape[0],
-            tables.shape[1], api._dev_ptr(refcounts), api._dev_ptr(tables), api._dev_ptr(lengths), api._dev_ptr(self.report),
-            api._dev_ptr(self._workspace), need.value)
+            ctypes.sizeof(_lib.PageCacheStruct), self._pointers, size // max(1, pages), len(pools), pages, page_tokens,
+            tables.shape[0], tables.shape[1], api._dev_ptr(refcounts), api._dev_ptr(tables), api._dev_ptr(lengths),
+            api._dev_ptr(self.report), api._dev_ptr(self._workspace), need.value)
         self._ref = ctypes.byref(self._struct)
+        self._lib = lib
 
     @classmethod
     def empty(cls, pools, page_tokens, sequences, pages_per_sequence):
@@ -161,39 +172,42 @@ class PageCache:
         return cls(pools, page_tokens, ints(0, pools[0].shape[0]), ints(-1, sequences, pages_per_sequence),
                    ints(0, sequences))
 
-    def _run(self, name, stream, *lists):
+    def _lists(self, *lists):
+        """Addresses of the lists, and their common length."""
+        n = lists[0].numel()
         for t in lists:
-            if t.dtype != torch.int32:
+            if t.dtype is not torch.int32:
                 raise TypeError("lists of sequences, pages and lengths are int32 tensors")
-            if t.numel() != lists[0].numel():
+            if t.numel() != n:
                 raise ValueError("the lists must agree in length")
-        _same_device(self.refcounts, *lists)
-        args = [api._dev_ptr(t) for t in lists] + ([lists[0].numel()] if lists else [])
-        _call(self.refcounts, getattr(self.lib, name), name, self._ref, *args, _stream_of(self.refcounts, stream))
+        _on(self._device, *lists)
+        return [api._dev_ptr(t) for t in lists] + [n]
 
     def copy(self, src_pages, dst_pages, source=None, stream=None):
         """Contents of the pages src_pages of `source` (default: this cache) into this cache's dst_pages, all pools."""
-        if src_pages.dtype != torch.int32 or dst_pages.dtype != torch.int32:
-            raise TypeError("lists of pages are int32 tensors")
-        if src_pages.numel() != dst_pages.numel():
-            raise ValueError("the lists must agree in length")
-        source = self if source is None else source
-        _same_device(self.refcounts, source.refcounts, src_pages, dst_pages)
-        _call(self.refcounts, self.lib.dfcclPagesCopy, "dfcclPagesCopy", self._ref, source._ref, api._dev_ptr(src_pages),
-              api._dev_ptr(dst_pages), src_pages.numel(), _stream_of(self.refcounts, stream))
+        lists = self._lists(src_pages, dst_pages)
+        if source is None:
+            source = self
+        elif source._device != self._device:
+            raise ValueError("the two caches must be on one device")
+        _call(self._device, self._lib.dfcclPagesCopy, "dfcclPagesCopy", self._ref, source._ref, *lists,
+              _stream_of(self._device, stream))
 
     def extend(self, sequences, lengths, stream=None):
         """The sequences grow to these lengths; new entries get the lowest free pages."""
-        self._run("dfcclPagesExtend", stream, sequences, lengths)
+        _call(self._device, self._lib.dfcclPagesExtend, "dfcclPagesExtend", self._ref, *self._lists(sequences, lengths),
+              _stream_of(self._device, stream))
 
     def fork(self, parents, children, stream=None):
         """The children (empty) become copies of the parents: full pages shared, a last page that is not full copied."""
-        self._run("dfcclPagesFork", stream, parents, children)
+        _call(self._device, self._lib.dfcclPagesFork, "dfcclPagesFork", self._ref, *self._lists(parents, children),
+              _stream_of(self._device, stream))
 
     def free(self, sequences, stream=None):
         """The sequences become empty and give up their pages."""
-        self._run("dfcclPagesFree", stream, sequences)
+        _call(self._device, self._lib.dfcclPagesFree, "dfcclPagesFree", self._ref, *self._lists(sequences),
+              _stream_of(self._device, stream))
 
     def compact(self, stream=None):
         """Moves pages until the live ones have the lowest numbers; counts and tables follow."""
-        self._run("dfcclPagesCompact", stream)
+        _call(self._device, self._lib.dfcclPagesCompact, "dfcclPagesCompact", self._ref, _stream_of(self._device, stream))

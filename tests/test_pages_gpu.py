@@ -152,9 +152,9 @@ def test_compact_full_empty_and_already_compact():
     both.compact()
 
 
-@pytest.mark.parametrize("pages", [127, 128, 512, 513, 1100, 5000])
+@pytest.mark.parametrize("pages", [127, 512, 513, 2047, 2100, 5000, 16384, 16385, 40000])
 def test_compact_and_extend_over_several_rounds_of_the_scan(pages):
-    if gpu_util.EMULATED and pages > 1100:
+    if gpu_util.EMULATED and pages > 2100:
         pytest.skip("too many emulated threads")
     rs = np.random.RandomState(pages)
     both = Both(pages=pages, page_tokens=1, sequences=40, per_seq=pages // 30, page_bytes=(4,), seed=1)
