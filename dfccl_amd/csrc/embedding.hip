@@ -81,7 +81,7 @@ __global__ __launch_bounds__(kRowThreads) void lookupKernel(LookupArgs a) {
         widen8<IN>(raw[u], f);
 #pragma unroll
         for (int i = 0; i < kVec; i++) f[i] = inside ? f[i] * a.scale : 0.0f;
-        store8<OUT>(a.out + (t0 + u) * a.outStride + (size_t)col * typeSize(OUT), f);
+        store8<OUT, OUT != kF32>(a.out + (t0 + u) * a.outStride + (size_t)col * typeSize(OUT), f);
       }
     } else if (col < a.width) {
       const int left = (int)(a.width - col);
@@ -174,7 +174,7 @@ __device__ __forceinline__ void clearShare(const Clear& c, uint32_t waves) {
     char* to = c.at + row * c.stride + part * kClearBytes;
     if (part + 1 < c.parts) {
 #pragma unroll
-      for (int u = 0; u < kClearStores; u++) store16<2>(to + (u * 64 + lane) * 16, zero);
+      for (int u = 0; u < kClearStores; u++) store16<2, true>(to + (u * 64 + lane) * 16, zero);
     } else {  // a row's last part, 1 .. kClearBytes bytes, an even number
       const uint32_t left = (uint32_t)(c.bytes - part * kClearBytes);
       for (uint32_t p = lane; p < left / 16; p += 64) store16<2>(to + p * 16, zero);
@@ -198,6 +198,16 @@ __device__ __forceinline__ void keyOfToken(const GradArgs& a, uint32_t pos, uint
   const int64_t id = loadId(ids, a.idBytes, t), row = rowOf(id, a.firstRow, a.rows);
   key = row >= 0 && id != a.paddingId ? (uint32_t)row : a.rows;
   pay = ((uint32_t)r << kSrcShift) | t;
+}
+__device__ __forceinline__ uint32_t payOf(const GradArgs& a, uint32_t pos) {
+  uint32_t r = 0, first = 0;
+#pragma unroll
+  for (int i = 1; i < kMaxSrcs; i++)
+    if (i < a.nsrcs && pos >= a.firstPos[i]) {
+      r = (uint32_t)i;
+      first = a.firstPos[i];
+    }
+  return (r << kSrcShift) | (pos - first);
 }
 
 // A strip's 64 keys of one wave: every lane's rank among the strip's keys of its digit, found with a ballot per bit,
@@ -230,33 +240,45 @@ __device__ __forceinline__ uint32_t waveScan(uint32_t v, int lane) {  // inclusi
   return v;
 }
 
-// ---- a few thousand tokens: sorted by one workgroup in LDS, one launch instead of two per digit
+// ---- up to some ten thousand tokens: sorted by one workgroup in LDS, one launch instead of two per digit
 constexpr int kSmallThreads = 1024;
 constexpr int kSmallWaves = kSmallThreads / 64;
-constexpr int kSmallStrips = 4;
-constexpr uint32_t kSmallMax = kSmallThreads * kSmallStrips;
+constexpr int kFewStrips = 4, kManyStrips = 16;
+// (a host build sets lower limits, to reach with few tokens what lies beyond them)
+#ifndef DFCCL_SORT_SMALL_MAX
+#define DFCCL_SORT_SMALL_MAX (kSmallThreads * kManyStrips)
+#endif
+#ifndef DFCCL_SUPER_MIN
+#define DFCCL_SUPER_MIN (256 * kChunk)
+#endif
+constexpr uint32_t kSmallMax = DFCCL_SORT_SMALL_MAX, kSuperMin = DFCCL_SUPER_MIN;
+static_assert(kSmallMax <= kSmallThreads * kManyStrips, "one workgroup sorts no more");
 constexpr int kSmallDigitBits = 8;
 constexpr int kSmallBins = 1 << kSmallDigitBits;
 
+template <int S>
 __global__ __launch_bounds__(kSmallThreads) void sortSmallKernel(GradArgs a, int keyBits, Clear c) {
   struct Shared {
-    uint32_t key[kSmallMax], pay[kSmallMax];
+    uint32_t key[kSmallThreads * S];
+    uint16_t pos[kSmallThreads * S];  // before sorting
     uint32_t count[kSmallWaves][kSmallBins];
     uint32_t waveTotal[kSmallBins / 64];
   };
+  static_assert(kSmallThreads * kManyStrips <= 65536, "positions are held in 16 bits");
   DFCCL_WG_SHARED(Shared, sh);
   if (blockIdx.x >= c.firstBlock) {
     clearShare(c, kSmallWaves);
     return;
   }
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = waveInBlock();
-  const uint32_t start = (uint32_t)wave * (64 * kSmallStrips);
-  uint32_t key[kSmallStrips], pay[kSmallStrips], rank[kSmallStrips];
+  const uint32_t start = (uint32_t)wave * (64 * S);
+  uint32_t key[S], pos[S], rank[S];
 #pragma unroll
-  for (int k = 0; k < kSmallStrips; k++) {
-    const uint32_t pos = start + k * 64 + lane;
-    key[k] = pay[k] = 0;
-    if (pos < a.n) keyOfToken(a, pos, key[k], pay[k]);
+  for (int k = 0; k < S; k++) {
+    uint32_t pay;
+    pos[k] = start + k * 64 + lane;
+    key[k] = 0;
+    if (pos[k] < a.n) keyOfToken(a, pos[k], key[k], pay);
   }
   const int passes = (keyBits + kSmallDigitBits - 1) / kSmallDigitBits, bits = (keyBits + passes - 1) / passes;
   for (int pass = 0; pass < passes; pass++) {
@@ -265,7 +287,7 @@ __global__ __launch_bounds__(kSmallThreads) void sortSmallKernel(GradArgs a, int
     for (int i = tid; i < kSmallWaves * kSmallBins; i += kSmallThreads) sh.count[i / kSmallBins][i % kSmallBins] = 0;
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kSmallStrips; k++)
+    for (int k = 0; k < S; k++)
       if (start + k * 64 < a.n)
         rank[k] = rankInWave(sh.count[wave], (key[k] >> shift) & mask, bits, start + k * 64 + lane < a.n, lane);
     __syncthreads();
@@ -290,28 +312,28 @@ __global__ __launch_bounds__(kSmallThreads) void sortSmallKernel(GradArgs a, int
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kSmallStrips; k++)
+    for (int k = 0; k < S; k++)
       if (start + k * 64 + lane < a.n) {
         const uint32_t to = sh.count[wave][(key[k] >> shift) & mask] + rank[k];
         sh.key[to] = key[k];
-        sh.pay[to] = pay[k];
+        sh.pos[to] = (uint16_t)pos[k];
       }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kSmallStrips; k++) {
-      const uint32_t pos = start + k * 64 + lane;
-      if (pos < a.n) {
-        key[k] = sh.key[pos];
-        pay[k] = sh.pay[pos];
+    for (int k = 0; k < S; k++) {
+      const uint32_t at = start + k * 64 + lane;
+      if (at < a.n) {
+        key[k] = sh.key[at];
+        pos[k] = sh.pos[at];
       }
     }
   }
 #pragma unroll
-  for (int k = 0; k < kSmallStrips; k++) {
-    const uint32_t pos = start + k * 64 + lane;
-    if (pos < a.n) {
-      a.keys[0][pos] = key[k];
-      a.pays[0][pos] = pay[k];
+  for (int k = 0; k < S; k++) {
+    const uint32_t at = start + k * 64 + lane;
+    if (at < a.n) {
+      a.keys[0][at] = key[k];
+      a.pays[0][at] = payOf(a, pos[k]);
     }
   }
 }
@@ -656,7 +678,7 @@ static GradPlan planGrad(uint64_t n, size_t rows, size_t width) {
   // Runs of fewer than 64 tokens need no chunks. Chunks of chunks pay for their launch once a run may have several
   // hundred chunks.
   p.chunked = n >= 64;
-  p.supered = n >= 256 * kChunk;
+  p.supered = n >= kSuperMin;
   size_t at = 0;
   auto take = [&at](size_t bytes) {
     const size_t here = at;
@@ -716,9 +738,9 @@ DFCCL_API ncclResult_t dfcclEmbeddingLookup(const void* table, ncclDataType_t ta
   a.pieces = (uint32_t)((width + kPieceElems - 1) / kPieceElems);
   a.idBytes = idType == ncclInt64 ? 8 : 4;
   a.scale = (float)scale;
-  constexpr int U = 4;
-  // four rows a wave once that still fills the chip (256 CUs, 32 waves each); below, one row a wave
-  const bool many = (uint64_t)tokens * a.pieces >= 4u * 256 * 32;
+  constexpr int U = 2;
+  // two rows a wave once that still fills the chip (256 CUs, 32 waves each); below, one row a wave
+  const bool many = (uint64_t)tokens * a.pieces >= (uint64_t)U * 256 * 32;
   const uint64_t waves = (uint64_t)((tokens + (many ? U : 1) - 1) / (many ? U : 1)) * a.pieces;
   LookupKernel fn = many ? pickLookup<U>((int)tableType, (int)outType) : pickLookup<1>((int)tableType, (int)outType);
   DFCCL_LAUNCH_BLOCKS(fn, gridFor(waves), kRowThreads, (hipStream_t)stream, a);
@@ -811,7 +833,8 @@ DFCCL_API ncclResult_t dfcclEmbeddingGrad(const void* const* grads, const void* 
   int from = 0;
   if (p.small) {
     const unsigned grid = share(1, kSmallWaves);
-    DFCCL_LAUNCH_BLOCKS(sortSmallKernel, grid, kSmallThreads, st, a, p.keyBits, clear);
+    DFCCL_LAUNCH_BLOCKS((n <= kSmallThreads * kFewStrips ? sortSmallKernel<kFewStrips> : sortSmallKernel<kManyStrips>), grid,
+                        kSmallThreads, st, a, p.keyBits, clear);
   }
   for (int pass = 0; !p.small && pass < p.passes; pass++, from ^= 1) {
     const SortPass s{from, pass * p.digitBits, p.digitBits, p.tiles};

@@ -49,9 +49,11 @@ template <int A>
 __device__ __forceinline__ u32x4 load16(const char* p) {
   return *(const DFCCL_GLOBAL typename Pack16<A>::type*)p;
 }
-template <int A>
+// NT: what is not read again soon does not stay in the caches
+template <int A, bool NT = false>
 __device__ __forceinline__ void store16(char* p, u32x4 v) {
-  *(DFCCL_GLOBAL typename Pack16<A>::type*)p = v;
+  if constexpr (NT) __builtin_nontemporal_store(v, (DFCCL_GLOBAL typename Pack16<A>::type*)p);
+  else *(DFCCL_GLOBAL typename Pack16<A>::type*)p = v;
 }
 
 __device__ __forceinline__ int waveInBlock() {  // the same in every lane: say so
@@ -131,7 +133,7 @@ __device__ __forceinline__ void widen8(const Raw8<DT>& r, float (&f)[kVec]) {
     for (int i = 0; i < 4; i++) widenWord<DT>(r.w[0][i], f[2 * i], f[2 * i + 1]);
   }
 }
-template <int DT>
+template <int DT, bool NT = false>
 __device__ __forceinline__ void store8(char* p, const float (&f)[kVec]) {
   u32x4 a;
   if constexpr (DT == kF32) {
@@ -141,12 +143,12 @@ __device__ __forceinline__ void store8(char* p, const float (&f)[kVec]) {
       a[i] = __float_as_uint(f[i]);
       b[i] = __float_as_uint(f[4 + i]);
     }
-    store16<4>(p, a);
-    store16<4>(p + 16, b);
+    store16<4, NT>(p, a);
+    store16<4, NT>(p + 16, b);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; i++) a[i] = narrowWord<DT>(f[2 * i], f[2 * i + 1]);
-    store16<2>(p, a);
+    store16<2, NT>(p, a);
   }
 }
 // the last, shorter vector of a row: `left` elements (1..7)

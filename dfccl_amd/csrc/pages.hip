@@ -28,6 +28,7 @@ constexpr int kScanPer = 4;  // counts a thread reads at once
 constexpr int kScanTile = kScanThreads * kScanPer;
 // Up to so many tiles one workgroup scans all pages; above, a workgroup per tile counts and another launch lists.
 constexpr int kOneScan = 4;
+constexpr int kFewRequests = 64;  // of an extend, carried out by the one workgroup that scans: a few for each of its waves
 
 // The bookkeeping as the kernels see it.
 struct Books {
@@ -156,9 +157,42 @@ __device__ __forceinline__ int32_t readRequests(ScanShared& sh, const Books& b, 
   return needed;
 }
 
-// A few tiles of pages: requests and free pages in one launch.
+__device__ __forceinline__ void refuse(const Books& b) {
+  if (b.report != nullptr) __hip_atomic_fetch_add(&b.report[0], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// One request of an extend, by `threads` threads: the new entries, their counts, the length.
+__device__ __forceinline__ void extendOne(const Books& b, const PageScratch& s, const Requests& q, int32_t i, int32_t foundPages,
+                                          int32_t thread, int32_t threads) {
+  const int32_t first = s.request[i];
+  int32_t have = 0, want = 0, seq = 0, length = 0;
+  bool met = false;
+  if (first >= 0) {
+    seq = q.a[i];
+    length = q.b[i];
+    have = pagesOf(s.before[i], b.pageTokens);
+    want = pagesOf(length, b.pageTokens);
+    met = want == have || first + (want - have) <= foundPages;
+  }
+  if (!met) {
+    if (thread == 0) refuse(b);
+    return;
+  }
+  int32_t* row = b.tables + (size_t)seq * b.perSeq;
+  for (int32_t k = have + thread; k < want; k += threads) {
+    const int32_t page = s.found[first + k - have];
+    row[k] = page;
+    b.refcounts[page] = 1;
+  }
+  if (thread == 0) b.lengths[seq] = length;
+}
+__global__ __launch_bounds__(kMoveThreads) void extendKernel(Books b, PageScratch s, Requests q) {
+  extendOne(b, s, q, (int32_t)blockIdx.x, s.counts[0], (int32_t)threadIdx.x, kMoveThreads);
+}
+
+// A few tiles of pages: requests and free pages in one launch, and an extend of a few sequences as a whole.
 template <bool FORK>
-__global__ __launch_bounds__(kScanThreads) void assignKernel(Books b, PageScratch s, Requests q) {
+__global__ __launch_bounds__(kScanThreads) void assignKernel(Books b, PageScratch s, Requests q, bool carryOut) {
   struct Shared {
     ScanShared scan;
   };
@@ -168,7 +202,13 @@ __global__ __launch_bounds__(kScanThreads) void assignKernel(Books b, PageScratc
   int which = 0;
   for (int64_t at = 0; at < b.pages && have < needed; at += kScanTile, which ^= 1)
     have += listFree(sh.scan, which, b, at, have, needed, s.found);
-  if (threadIdx.x == 0) s.counts[0] = (int32_t)(have < needed ? have : needed);
+  const int32_t foundPages = (int32_t)(have < needed ? have : needed);
+  if (threadIdx.x == 0) s.counts[0] = foundPages;
+  if constexpr (!FORK) {
+    if (!carryOut) return;
+    __syncthreads();
+    for (int32_t i = waveInBlock(); i < q.n; i += kScanWaves) extendOne(b, s, q, i, foundPages, (int32_t)(threadIdx.x & 63), 64);
+  }
 }
 
 // Many tiles, first launch: workgroup 0 reads the requests (a compaction has none), the others count a tile each.
@@ -218,37 +258,6 @@ __global__ __launch_bounds__(kScanThreads) void listFreeKernel(Books b, PageScra
   if (have < needed) (void)listFree(sh.scan, 1, b, (int64_t)tile * kScanTile, have, needed, s.found);
 }
 
-__device__ __forceinline__ void refuse(const Books& b) {
-  if (b.report != nullptr) __hip_atomic_fetch_add(&b.report[0], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
-// One workgroup per request of an extend: the new entries, their counts, the length.
-__global__ __launch_bounds__(kMoveThreads) void extendKernel(Books b, PageScratch s, Requests q) {
-  for (int32_t i = (int32_t)blockIdx.x; i < q.n; i += (int32_t)gridDim.x) {
-    const int32_t first = s.request[i];
-    int32_t have = 0, want = 0, seq = 0, length = 0;
-    bool met = false;
-    if (first >= 0) {
-      seq = q.a[i];
-      length = q.b[i];
-      have = pagesOf(s.before[i], b.pageTokens);
-      want = pagesOf(length, b.pageTokens);
-      met = want == have || first + (want - have) <= s.counts[0];
-    }
-    if (!met) {
-      if (threadIdx.x == 0) refuse(b);
-      continue;
-    }
-    int32_t* row = b.tables + (size_t)seq * b.perSeq;
-    for (int32_t k = have + (int32_t)threadIdx.x; k < want; k += kMoveThreads) {
-      const int32_t page = s.found[first + k - have];
-      row[k] = page;
-      b.refcounts[page] = 1;
-    }
-    if (threadIdx.x == 0) b.lengths[seq] = length;
-  }
-}
-
 // ---- contents
 
 struct PoolSet {
@@ -269,7 +278,7 @@ __device__ __forceinline__ void movePart(const char* from, char* to, uint32_t by
 #pragma unroll
     for (int u = 0; u < kPartLoads; u++) v[u] = load16<1>(from + (u * 64 + lane) * 16);
 #pragma unroll
-    for (int u = 0; u < kPartLoads; u++) store16<1>(to + (u * 64 + lane) * 16, v[u]);
+    for (int u = 0; u < kPartLoads; u++) store16<1, true>(to + (u * 64 + lane) * 16, v[u]);
     return;
   }
   const uint32_t packs = bytes / 16;
@@ -277,27 +286,37 @@ __device__ __forceinline__ void movePart(const char* from, char* to, uint32_t by
   for (uint32_t i = packs * 16 + lane; i < bytes; i += 64)
     ((DFCCL_GLOBAL char*)to)[i] = ((const DFCCL_GLOBAL char*)from)[i];
 }
-// item = (pair, pool, part) of a move, numbered so that neighbours touch neighbouring memory
-__device__ __forceinline__ void moveItem(const PoolSet& p, int32_t src, int32_t dst, uint32_t inPair, int lane) {
-  const uint32_t pool = inPair / p.parts, part = inPair % p.parts;
-  const size_t at = (size_t)part * kPartBytes;
+// The items of n moves: (pool, move, part), numbered so that neighbours touch neighbouring memory of one pool.
+struct MoveItem {
+  uint32_t pool, move, part;
+};
+__device__ __forceinline__ MoveItem itemOf(const PoolSet& p, uint64_t item, uint32_t n) {
+  const uint64_t perPool = (uint64_t)n * p.parts;
+  MoveItem m;
+  m.pool = (uint32_t)(item / perPool);
+  const uint64_t in = item - m.pool * perPool;
+  m.move = (uint32_t)(in / p.parts);
+  m.part = (uint32_t)(in - (uint64_t)m.move * p.parts);
+  return m;
+}
+__device__ __forceinline__ void moveItem(const PoolSet& p, int32_t src, int32_t dst, const MoveItem& m, int lane) {
+  const size_t at = (size_t)m.part * kPartBytes;
   // (the last part's size comes from the host: the minimum of two 64-bit sizes that are the same in every lane is
   // compiled into a vector compare whose result the scalar select that follows does not read)
-  const uint32_t bytes = part + 1 == p.parts ? p.lastBytes : kPartBytes;
-  movePart(p.from[pool] + (size_t)src * p.pageBytes + at, p.to[pool] + (size_t)dst * p.pageBytes + at, bytes, (uint32_t)lane);
+  const uint32_t bytes = m.part + 1 == p.parts ? p.lastBytes : kPartBytes;
+  movePart(p.from[m.pool] + (size_t)src * p.pageBytes + at, p.to[m.pool] + (size_t)dst * p.pageBytes + at, bytes, (uint32_t)lane);
 }
 
 __global__ __launch_bounds__(kMoveThreads) void copyKernel(PoolSet p, const int32_t* srcPages, const int32_t* dstPages,
                                                            int32_t n, int32_t srcTotal, int32_t dstTotal) {
   const int lane = (int)(threadIdx.x & 63);
-  const uint32_t perPair = (uint32_t)p.npools * p.parts;
-  const uint64_t items = (uint64_t)n * perPair;
+  const uint64_t items = (uint64_t)n * p.npools * p.parts;
   for (uint64_t item = (uint64_t)blockIdx.x * kMoveWaves + waveInBlock(); item < items;
        item += (uint64_t)gridDim.x * kMoveWaves) {
-    const uint32_t i = (uint32_t)(item / perPair);
-    const int32_t src = uniform(srcPages[i]), dst = uniform(dstPages[i]);
+    const MoveItem m = itemOf(p, item, (uint32_t)n);
+    const int32_t src = uniform(srcPages[m.move]), dst = uniform(dstPages[m.move]);
     if (src < 0 || src >= srcTotal || dst < 0 || dst >= dstTotal) continue;
-    moveItem(p, src, dst, (uint32_t)(item % perPair), lane);
+    moveItem(p, src, dst, m, lane);
   }
 }
 
@@ -332,16 +351,15 @@ __global__ __launch_bounds__(kMoveThreads) void forkKernel(Books b, PageScratch 
     return;
   }
   const int lane = (int)(threadIdx.x & 63);
-  const uint32_t perPair = (uint32_t)p.npools * p.parts;
-  const uint64_t items = (uint64_t)q.n * perPair;
+  const uint64_t items = (uint64_t)q.n * p.npools * p.parts;
   for (uint64_t item = (uint64_t)(blockIdx.x - tableBlocks) * kMoveWaves + waveInBlock(); item < items;
        item += (uint64_t)(gridDim.x - tableBlocks) * kMoveWaves) {
-    const uint32_t i = (uint32_t)(item / perPair);
-    const int32_t first = uniform(s.request[i]), before = uniform(s.before[i]);
+    const MoveItem m = itemOf(p, item, (uint32_t)q.n);
+    const int32_t first = uniform(s.request[m.move]), before = uniform(s.before[m.move]);
     if (first < 0 || before % b.pageTokens == 0 || first >= uniform(s.counts[0])) continue;
-    const int32_t src = uniform(b.tables[(size_t)uniform(q.a[i]) * b.perSeq + before / b.pageTokens]);
+    const int32_t src = uniform(b.tables[(size_t)uniform(q.a[m.move]) * b.perSeq + before / b.pageTokens]);
     if (src < 0 || src >= b.pages) continue;
-    moveItem(p, src, uniform(s.found[first]), (uint32_t)(item % perPair), lane);
+    moveItem(p, src, uniform(s.found[first]), m, lane);
   }
 }
 
@@ -500,12 +518,11 @@ __global__ __launch_bounds__(kMoveThreads) void compactKernel(Books b, PageScrat
     return;
   }
   const int lane = (int)(threadIdx.x & 63);
-  const uint32_t perPair = (uint32_t)p.npools * p.parts;
-  const uint64_t items = (uint64_t)moves * perPair;
+  const uint64_t items = (uint64_t)moves * p.npools * p.parts;
   for (uint64_t item = (uint64_t)(blockIdx.x - bookBlocks) * kMoveWaves + waveInBlock(); item < items;
        item += (uint64_t)(gridDim.x - bookBlocks) * kMoveWaves) {
-    const uint32_t i = (uint32_t)(item / perPair);
-    moveItem(p, uniform(s.movers[i]), uniform(s.found[i]), (uint32_t)(item % perPair), lane);
+    const MoveItem m = itemOf(p, item, (uint32_t)moves);
+    moveItem(p, uniform(s.movers[m.move]), uniform(s.found[m.move]), m, lane);
   }
 }
 
@@ -593,14 +610,18 @@ constexpr uint64_t kMaxMoveGrid = 1u << 22;
 static unsigned moveGrid(uint64_t items) {
   return (unsigned)std::max<uint64_t>(1, std::min<uint64_t>((items + kMoveWaves - 1) / kMoveWaves, kMaxMoveGrid));
 }
+// Returns whether that has carried the requests out, too.
 template <int FOR>
-static void launchAssign(const Books& b, const PageScratch& s, const Requests& q, hipStream_t st) {
+static bool launchAssign(const Books& b, const PageScratch& s, const Requests& q, hipStream_t st) {
   const int32_t tiles = (int32_t)tilesOf(b.pages);
+  const bool few = FOR == kForExtend && q.n <= kFewRequests;
   if (tiles <= kOneScan) {
-    DFCCL_LAUNCH_BLOCKS(assignKernel<FOR == kForFork>, 1, kScanThreads, st, b, s, q);
+    DFCCL_LAUNCH_BLOCKS(assignKernel<FOR == kForFork>, 1, kScanThreads, st, b, s, q, few);
+    return few;
   } else {
     DFCCL_LAUNCH_BLOCKS(countTilesKernel<FOR>, (unsigned)tiles + 1, kScanThreads, st, b, s, q);
     DFCCL_LAUNCH_BLOCKS(listFreeKernel, (unsigned)tiles, kScanThreads, st, b, s, tiles);
+    return false;
   }
 }
 static ncclResult_t launched() { return hipGetLastError() == hipSuccess ? ncclSuccess : ncclUnhandledCudaError; }
@@ -641,8 +662,8 @@ DFCCL_API ncclResult_t dfcclPagesExtend(const dfcclPageCache* c, const int32_t* 
   const hipStream_t st = (hipStream_t)stream;
   const PageScratch s = scratchOf(c);
   const Requests q{sequences, lengths, n};
-  launchAssign<kForExtend>(b, s, q, st);
-  if (n > 0) DFCCL_LAUNCH_BLOCKS(extendKernel, (unsigned)n, kMoveThreads, st, b, s, q);
+  const bool done = launchAssign<kForExtend>(b, s, q, st);
+  if (n > 0 && !done) DFCCL_LAUNCH_BLOCKS(extendKernel, (unsigned)n, kMoveThreads, st, b, s, q);
   return launched();
 }
 
@@ -654,7 +675,7 @@ DFCCL_API ncclResult_t dfcclPagesFork(const dfcclPageCache* c, const int32_t* pa
   const hipStream_t st = (hipStream_t)stream;
   const PageScratch s = scratchOf(c);
   const Requests q{parents, children, n};
-  launchAssign<kForFork>(b, s, q, st);
+  (void)launchAssign<kForFork>(b, s, q, st);
   for (int first = 0; n > 0 && first < c->npools; first += kMaxPools) {
     const PoolSet p = poolSet(c, c, first);
     const unsigned tableBlocks = first == 0 ? (unsigned)n : 0u;

@@ -41,7 +41,7 @@ def _rows_ptr(t, what):
     if t.dtype not in _FLOATS:
         raise TypeError(f"{what}: dtype {t.dtype} is not one of float32, float16, bfloat16")
     if t.is_contiguous():
-        return api._dev_ptr(t), t.shape[1]
+        return t.data_ptr() if t.is_cuda else api._dev_ptr(t), t.shape[1]
     if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
         raise ValueError(f"{what}: the elements of a row must be contiguous, and rows must not overlap")
     return api._dev_ptr(t[0]), t.stride(0) if t.shape[0] > 1 else t.shape[1]

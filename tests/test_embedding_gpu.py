@@ -186,6 +186,15 @@ def test_grad_of_one_token_many_times(tokens, accumulate):
           accumulate=accumulate)
 
 
+@big_only
+@pytest.mark.parametrize("tokens", [8191, 8192, 8193, 20000, 33000])
+def test_grad_of_one_token_thousands_of_times(tokens):
+    for ahead in (0, 45):
+        ids = torch.full((tokens + ahead,), 3, device="cuda:0")
+        ids[:ahead] = 1
+        _grad([_randn(24, tokens + ahead, 24)], [ids], 5, torch.float32)
+
+
 @pytest.mark.parametrize("ahead", [0, 1, 17, 32, 40])
 def test_grad_of_long_runs_that_begin_anywhere(ahead):
     ids = torch.cat([torch.full((n,), v) for v, n in ((0, ahead), (2, 1100), (3, 1), (4, 64), (6, 2100))])
@@ -260,10 +269,11 @@ def test_grad_row_counts_around_the_digits_of_the_sort(rows):
     _grad([_randn(53, 400, 9)], [ids], rows, torch.float32)
 
 
-def test_grad_sorts_over_several_tiles():
-    # 1024 tokens a tile: five tiles, ids that differ in both digits
-    ids = _ids(54, 4500, 0, 1500)
-    _grad([_randn(55, 4500, 8)], [ids], 1500, torch.float32, accumulate=True)
+@pytest.mark.parametrize("tokens", [4097, 5100] + ([] if gpu_util.EMULATED else [16384, 16385, 40000]))
+def test_grad_sorts_by_one_workgroup_and_over_several_tiles(tokens):
+    # 4096 and 16384 tokens are the limits of a workgroup's two ways (the host build has its second one at 5000)
+    ids = _ids(54, tokens, 0, 1500)
+    _grad([_randn(55, tokens, 8)], [ids], 1500, torch.float32, accumulate=tokens % 2 == 0)
 
 
 @big_only
