@@ -117,10 +117,10 @@ static LookupKernel pickLookup(int in, int out) {
 // 2. Chunks. The sorted list is cut into chunks of kChunk. A chunk that lies within one row's run is summed by a
 //    wave of its own into fp32 scratch, and so are kChunk such chunks: a row that many tokens share (padding that
 //    counts, frequent words) is summed by many waves, and again in a fixed order.
-// 3. Rows. A wave per sorted position and row piece goes on where its position begins a run: single tokens up to the
-//    first whole chunk, whole chunks' (and chunks of chunks') sums, single tokens after the last.
+// 3. Rows. A wave per group of sorted positions and row piece sums the runs that begin in its group: single tokens up to
+//    the first whole chunk, whole chunks' (and chunks of chunks') sums, single tokens after the last.
 // Without accumulation the rows that no token names have to become zeros. That is most of the table and most of the
-// bytes, and it needs nothing of the sort: all rows are cleared by additional workgroups of the launches of 1. and 2.,
+// bytes, and it needs nothing of the sort: all rows are cleared by additional workgroups of the launches of 1.,
 // which leave most of the chip idle, and the named rows are written over afterwards.
 
 constexpr int kChunk = 32;
@@ -153,33 +153,50 @@ struct SortPass {
   int from, shift, bits, tiles;  // keys[from] -> keys[from ^ 1]
 };
 
-// A share of the clearing of the table: parts [begin, end) of rows of `bytes` bytes, each row in `parts` parts.
-// (A table without gaps between its rows is one long row.)
+// A share of the clearing of the table: parts [begin, end), done by the launch's workgroups from firstBlock on. A table
+// without gaps between its rows is cleared as one range, a part being what a workgroup stores at once; otherwise a part
+// is kGapBytes of one row, by a wave.
 struct Clear {
   char* at;
-  size_t stride;
-  uint64_t bytes, parts, begin, end;
-  uint32_t firstBlock;  // the launch's workgroups from here on clear
+  size_t stride;        // of the rows, 0 for one range
+  uint64_t bytes;       // of a row, or of the range
+  uint64_t rowParts;    // of a row
+  uint64_t begin, end;
+  uint32_t firstBlock;
 };
-constexpr int kClearStores = 4;
-constexpr uint32_t kClearBytes = 64 * 16 * kClearStores;  // of a part
-constexpr unsigned kClearWavesPerCu = 16;
+// How a workgroup clears a range, from a sweep over 1 GiB: workgroups of 4 waves that store 16 bytes a thread once and
+// end reach 7.0 TB/s (four stores a thread 6.1, a fixed number of workgroups that walk the range 4.9 to 5.4); a
+// workgroup of 16 waves that has its compute unit to itself walks the range with eight stores a thread, each 16 KiB of
+// the workgroup in one piece (6.5 TB/s; four stores 6.1, each wave's stores in one piece 5.6).
+constexpr uint32_t clearStores(uint32_t waves) { return waves >= 16 ? 8 : 1; }
+constexpr uint32_t clearPart(uint32_t waves) { return waves * clearStores(waves) * 1024; }
+constexpr uint32_t kGapBytes = 4096;
 
-__device__ __forceinline__ void clearShare(const Clear& c, uint32_t waves) {
-  const uint32_t lane = threadIdx.x & 63, blocks = gridDim.x - c.firstBlock;
+template <uint32_t WAVES>
+__device__ __forceinline__ void clearShare(const Clear& c) {
+  const uint32_t lane = threadIdx.x & 63, blocks = gridDim.x - c.firstBlock, block = blockIdx.x - c.firstBlock;
   const u32x4 zero = {0, 0, 0, 0};
-  for (uint64_t i = c.begin + (uint64_t)(blockIdx.x - c.firstBlock) * waves + (uint32_t)waveInBlock(); i < c.end;
-       i += (uint64_t)blocks * waves) {
-    const uint64_t row = i / c.parts, part = i % c.parts;
-    char* to = c.at + row * c.stride + part * kClearBytes;
-    if (part + 1 < c.parts) {
+  if (c.stride == 0) {
+    constexpr uint32_t part = clearPart(WAVES);
+    for (uint64_t i = c.begin + block; i < c.end; i += blocks) {
+      char* to = c.at + i * part;
+      const uint64_t left = c.bytes - i * part;
+      if (left >= part) {
 #pragma unroll
-      for (int u = 0; u < kClearStores; u++) store16<2, true>(to + (u * 64 + lane) * 16, zero);
-    } else {  // a row's last part, 1 .. kClearBytes bytes, an even number
-      const uint32_t left = (uint32_t)(c.bytes - part * kClearBytes);
-      for (uint32_t p = lane; p < left / 16; p += 64) store16<2>(to + p * 16, zero);
-      for (uint32_t p = left / 16 * 8 + lane; p < left / 2; p += 64) storeElem<2>(to, p, 0);
+        for (uint32_t u = 0; u < clearStores(WAVES); u++) store16<2>(to + (u * WAVES * 64 + threadIdx.x) * 16, zero);
+      } else {  // the range's last bytes, an even number
+        for (uint32_t p = threadIdx.x; p < (uint32_t)left / 16; p += WAVES * 64) store16<2>(to + p * 16, zero);
+        for (uint32_t p = (uint32_t)left / 16 * 8 + threadIdx.x; p < (uint32_t)left / 2; p += WAVES * 64) storeElem<2>(to, p, 0);
+      }
     }
+    return;
+  }
+  for (uint64_t i = c.begin + (uint64_t)block * WAVES + (uint32_t)waveInBlock(); i < c.end; i += (uint64_t)blocks * WAVES) {
+    const uint64_t row = i / c.rowParts, part = i - row * c.rowParts;
+    char* to = c.at + row * c.stride + part * kGapBytes;
+    const uint32_t left = part + 1 < c.rowParts ? kGapBytes : (uint32_t)(c.bytes - part * kGapBytes);
+    for (uint32_t p = lane; p < left / 16; p += 64) store16<2>(to + p * 16, zero);
+    for (uint32_t p = left / 16 * 8 + lane; p < left / 2; p += 64) storeElem<2>(to, p, 0);
   }
 }
 
@@ -267,7 +284,7 @@ __global__ __launch_bounds__(kSmallThreads) void sortSmallKernel(GradArgs a, int
   static_assert(kSmallThreads * kManyStrips <= 65536, "positions are held in 16 bits");
   DFCCL_WG_SHARED(Shared, sh);
   if (blockIdx.x >= c.firstBlock) {
-    clearShare(c, kSmallWaves);
+    clearShare<kSmallWaves>(c);
     return;
   }
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = waveInBlock();
@@ -352,7 +369,7 @@ __global__ __launch_bounds__(kSortThreads) void sortCountKernel(GradArgs a, Sort
   };
   DFCCL_WG_SHARED(Shared, sh);
   if (blockIdx.x >= c.firstBlock) {
-    clearShare(c, kSortWaves);
+    clearShare<kSortWaves>(c);
     return;
   }
   const int tid = (int)threadIdx.x, tile = (int)blockIdx.x, bins = 1 << p.bits;
@@ -384,7 +401,7 @@ __global__ __launch_bounds__(kSortThreads) void sortScatterKernel(GradArgs a, So
   };
   DFCCL_WG_SHARED(Shared, sh);
   if (blockIdx.x >= c.firstBlock) {
-    clearShare(c, kSortWaves);
+    clearShare<kSortWaves>(c);
     return;
   }
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = waveInBlock(), tile = (int)blockIdx.x, bins = 1 << p.bits;
@@ -454,44 +471,64 @@ __global__ __launch_bounds__(kSortThreads) void sortScatterKernel(GradArgs a, So
 
 // ---- sums
 
-// acc += the gradients of `count` tokens (at most 64) whose payloads lanes from .. from + count - 1 hold, this lane's
-// eight columns, in order. The payloads come by lane, so the loads depend on nothing but each other's registers:
-// kAhead of them are in flight.
-template <int GT>
-__device__ __forceinline__ void addTokens(const GradArgs& a, uint32_t pays, int from, int count, uint32_t col,
-                                          float (&acc)[kVec]) {
-  constexpr int kAhead = GT == kF32 ? 8 : 16;
-  const int left = (int)a.width - (int)col;
-  for (int p = 0; p < count; p += kAhead) {
-    Raw8<GT> raw[kAhead];
-#pragma unroll
-    for (int i = 0; i < kAhead; i++)
-      if (p + i < count) {
-        const uint32_t pay = (uint32_t)__builtin_amdgcn_readlane((int)pays, from + p + i);
-        const char* row = a.grads[pay >> kSrcShift] + (size_t)(pay & kTokenMask) * a.gradStride;
-        if (left >= kVec) {
-          raw[i] = loadRaw8<GT>(row + (size_t)col * typeSize(GT));
-        } else if (left > 0) {  // (the last, shorter vector of a row, put together from elements)
-          raw[i] = Raw8<GT>{};
-#pragma unroll
-          for (int j = 0; j < kVec - 1; j++)
-            if (j < left) {
-              const uint32_t e = (uint32_t)loadElem<typeSize(GT)>(row + (size_t)col * typeSize(GT), j);
-              if constexpr (GT == kF32) raw[i].w[j / 4][j % 4] = e;
-              else raw[i].w[0][j / 2] |= e << (16 * (j % 2));
-            }
-        }
-      }
-    if (left > 0) {
-#pragma unroll
-      for (int i = 0; i < kAhead; i++)
-        if (p + i < count) {
-          float f[kVec];
-          widen8<GT>(raw[i], f);
-#pragma unroll
-          for (int j = 0; j < kVec; j++) acc[j] += f[j];
-        }
+// A lane's eight columns of a row of a.width elements. The last lane's would reach beyond the row's end unless the width
+// is a multiple of eight: it takes the row's last eight elements instead, `shift` of which are the lane's before, and
+// only stores its own. A row of fewer than eight elements is put together from them.
+struct Columns {
+  uint32_t at, slot;  // first column that is loaded; place in fp32 scratch (which has whole vectors)
+  int count, shift;   // elements there (8, fewer in a narrow row, 0 beyond the row); how many of them are not the lane's
+};
+__device__ __forceinline__ Columns columnsOf(uint32_t width, uint32_t piece, int lane) {
+  Columns c;
+  c.slot = piece * kPieceElems + (uint32_t)lane * kVec;
+  const int left = (int)width - (int)c.slot;
+  c.shift = left > 0 && left < kVec && width >= kVec ? kVec - left : 0;
+  c.at = c.slot - (uint32_t)c.shift;
+  c.count = left <= 0 ? 0 : left + c.shift < kVec ? left + c.shift : kVec;
+  return c;
+}
+template <int DT>
+__device__ __forceinline__ Raw8<DT> loadColumns(const char* row, const Columns& c) {
+  const char* p = row + (size_t)c.at * typeSize(DT);
+  if (c.count == kVec) return loadRaw8<DT>(p);
+  Raw8<DT> r{};
+#pragma unroll 1
+  for (int j = c.count - 1; j >= 0; j--) {  // (in from the low end)
+    const uint32_t e = (uint32_t)loadElem<typeSize(DT)>(p, j);
+    u32x4 w = r.w[0];
+    if constexpr (DT == kF32) {
+      u32x4 h = r.w[1];
+      r.w[1] = u32x4{w.w, h.x, h.y, h.z};
+      r.w[0] = u32x4{e, w.x, w.y, w.z};
+    } else {
+      r.w[0] = u32x4{(w.x << 16) | e, (w.y << 16) | (w.x >> 16), (w.z << 16) | (w.y >> 16), (w.w << 16) | (w.z >> 16)};
     }
+  }
+  return r;
+}
+template <int GT>
+__device__ __forceinline__ Raw8<GT> loadGradient(const GradArgs& a, uint32_t pay, const Columns& c) {
+  return loadColumns<GT>(a.grads[pay >> kSrcShift] + (size_t)(pay & kTokenMask) * a.gradStride, c);
+}
+
+// acc += the gradients of `count` tokens whose payloads lanes from .. from + count - 1 hold, this lane's eight columns,
+// in order. The payloads come by lane, so the loads depend on nothing but each other's registers: AHEAD are in flight.
+template <int GT, int AHEAD>
+__device__ __forceinline__ void addTokens(const GradArgs& a, uint32_t pays, int from, int count, const Columns& c,
+                                          float (&acc)[kVec]) {
+  for (int p = 0; p < count; p += AHEAD) {
+    Raw8<GT> raw[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++)
+      if (p + i < count) raw[i] = loadGradient<GT>(a, (uint32_t)__builtin_amdgcn_readlane((int)pays, from + p + i), c);
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++)
+      if (p + i < count) {
+        float f[kVec];
+        widen8<GT>(raw[i], f);
+#pragma unroll
+        for (int j = 0; j < kVec; j++) acc[j] += f[j];
+      }
   }
 }
 // acc += rows [begin, end) of fp32 scratch
@@ -517,24 +554,20 @@ __device__ __forceinline__ void addSums(const float* sums, uint32_t widthPad, ui
 
 // One wave per (chunk, piece): the chunk's sum if all of it belongs to one row.
 template <int GT>
-__global__ __launch_bounds__(kRowThreads) void chunkKernel(GradArgs a, int sorted, Clear c) {
-  if (blockIdx.x >= c.firstBlock) {
-    clearShare(c, kRowWaves);
-    return;
-  }
+__global__ __launch_bounds__(kRowThreads) void chunkKernel(GradArgs a, int sorted) {
   const int lane = (int)(threadIdx.x & 63);
   const uint32_t* keys = a.keys[sorted];
   const uint64_t items = (uint64_t)(a.n / kChunk) * a.pieces;
   for (uint64_t item = (uint64_t)blockIdx.x * kRowWaves + waveInBlock(); item < items;
-       item += (uint64_t)c.firstBlock * kRowWaves) {
+       item += (uint64_t)gridDim.x * kRowWaves) {
     const uint32_t chunk = (uint32_t)(item / a.pieces), piece = (uint32_t)(item % a.pieces), begin = chunk * kChunk;
     const uint32_t first = keys[begin], last = keys[begin + kChunk - 1], pays = a.pays[sorted][begin + (lane & (kChunk - 1))];
     const uint32_t key = uniform(first);
     if (key >= a.rows || uniform(last) != key) continue;
-    const uint32_t col = piece * kPieceElems + lane * kVec;
+    const Columns cols = columnsOf(a.width, piece, lane);
     float acc[kVec] = {};
-    addTokens<GT>(a, pays, 0, kChunk, col, acc);
-    if (col < a.widthPad) store8<kF32>((char*)(a.chunkSums + (size_t)chunk * a.widthPad + col), acc);
+    addTokens<GT, GT == kF32 ? 8 : 16>(a, pays, 0, kChunk, cols, acc);
+    if (cols.count > 0) store8<kF32>((char*)(a.chunkSums + (size_t)chunk * a.widthPad + cols.slot), acc);
   }
 }
 // One wave per (chunk of chunks, piece)
@@ -570,70 +603,109 @@ __device__ __forceinline__ uint32_t endOfRun(const uint32_t* keys, uint32_t key,
   return lo;
 }
 
-template <int TT>
-__device__ __forceinline__ void writeRow(const GradArgs& a, uint32_t row, uint32_t col, float (&acc)[kVec]) {
-  char* to = a.table + (size_t)row * a.tableStride + (size_t)col * typeSize(TT);
-  const int left = (int)a.width - (int)col;
-#pragma unroll
-  for (int j = 0; j < kVec; j++) acc[j] *= a.scale;
-  if (left >= kVec) {
-    if (a.accumulate) {
-      float old[kVec];
-      widen8<TT>(loadRaw8<TT>(to), old);
-#pragma unroll
-      for (int j = 0; j < kVec; j++) acc[j] += old[j];
-    }
-    store8<TT>(to, acc);
-  } else if (left > 0) {
-    if (a.accumulate) {
-      float old[kVec];
-      loadTail<TT>(to, left, old);
-#pragma unroll
-      for (int j = 0; j < kVec; j++) acc[j] += old[j];
-    }
-    storeTail<TT>(to, left, acc);
-  }
-}
+// One wave per (group of kGroup sorted positions, piece): the runs that begin in the group. A lane each reads the keys
+// from the one before the group on and the payloads from the group's first on, so after one load it is known where
+// runs begin and end and whom they sum; then the group's rows (and the table's, if they are added to) are in flight
+// together. Only the group's last run may go on behind it.
+constexpr int kGroup = 4;
+static_assert(kChunk % kGroup == 0, "a group lies within one chunk");
 
-template <int GT, int TT>
+template <int GT, int TT, bool ADD>
 __global__ __launch_bounds__(kRowThreads) void rowsKernel(GradArgs a, int sorted) {
   const int lane = (int)(threadIdx.x & 63);
   const uint32_t *keys = a.keys[sorted], *pays = a.pays[sorted];
-  const uint64_t items = (uint64_t)a.n * a.pieces;
+  const uint64_t items = (uint64_t)((a.n + (kGroup - 1)) / kGroup) * a.pieces;
   for (uint64_t item = (uint64_t)blockIdx.x * kRowWaves + waveInBlock(); item < items;
        item += (uint64_t)gridDim.x * kRowWaves) {
-    const uint32_t pos = (uint32_t)(item / a.pieces);
-    // the keys from the one before on, and the payloads from this one on, a lane each: whether a run begins here,
-    // where it ends and whom it sums is known after one load
-    const uint64_t at = (uint64_t)pos + (uint32_t)lane;
-    const uint32_t window = at >= 1 && at - 1 < a.n ? keys[at - 1] : a.rows;
-    const uint32_t mine = at < a.n ? pays[at] : 0;
-    const uint32_t key = (uint32_t)__builtin_amdgcn_readlane((int)window, 1);
-    const uint32_t prev = (uint32_t)__builtin_amdgcn_readlane((int)window, 0);
-    if (key >= a.rows || prev == key) continue;
-    const uint64_t same = __ballot(window == key) >> 1;  // bit i: position pos + i
-    uint32_t end = pos + (uint32_t)__builtin_ctzll(~same);
-    if (end - pos == 63) end = endOfRun(keys, key, end, a.n, lane);
-    const uint32_t col = (uint32_t)(item % a.pieces) * kPieceElems + (uint32_t)lane * kVec;
-    const uint32_t c0 = (pos + kChunk - 1) / kChunk, c1 = end / kChunk;
-    float acc[kVec] = {};
-    if (!a.chunked || c0 >= c1) {  // (fewer than 64 tokens either way)
-      addTokens<GT>(a, mine, 0, (int)(end - pos), col, acc);
-    } else {
-      const uint64_t behind = (uint64_t)c1 * kChunk + (uint32_t)lane;
-      const uint32_t rest = behind < end ? pays[behind] : 0;
-      addTokens<GT>(a, mine, 0, (int)(c0 * kChunk - pos), col, acc);
-      const uint32_t s0 = (c0 + kChunk - 1) / kChunk, s1 = c1 / kChunk;
-      if (!a.supered || s0 >= s1) {
-        addSums(a.chunkSums, a.widthPad, c0, c1, col, acc);
-      } else {
-        addSums(a.chunkSums, a.widthPad, c0, s0 * kChunk, col, acc);
-        addSums(a.superSums, a.widthPad, s0, s1, col, acc);
-        addSums(a.chunkSums, a.widthPad, s1 * kChunk, c1, col, acc);
-      }
-      addTokens<GT>(a, rest, 0, (int)(end - c1 * kChunk), col, acc);
+    const uint64_t group = item / a.pieces;
+    const Columns cols = columnsOf(a.width, (uint32_t)(item - group * a.pieces), lane);
+    const uint32_t p0 = (uint32_t)group * kGroup;
+    const uint64_t at = (uint64_t)p0 + (uint32_t)lane;
+    const uint32_t window = at >= 1 && at - 1 < a.n ? keys[at - 1] : a.rows;  // lane l: position p0 - 1 + l
+    const uint32_t mine = at < a.n ? pays[at] : 0;                            // lane l: position p0 + l
+    uint32_t key[kGroup + 1];
+    bool begins[kGroup], ours[kGroup];  // ours: of a run that begins in the group
+    uint32_t before = (uint32_t)__builtin_amdgcn_readlane((int)window, 0);
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i <= kGroup; i++) key[i] = (uint32_t)__builtin_amdgcn_readlane((int)window, i + 1);
+#pragma unroll
+    for (int i = 0; i < kGroup; i++) {
+      begins[i] = key[i] < a.rows && key[i] != before;
+      ours[i] = begins[i] || (any && key[i] < a.rows);  // (a run that began in the group goes on, or another begins)
+      any = any || begins[i];
+      before = key[i];
     }
-    writeRow<TT>(a, key, col, acc);
+    if (!any) continue;
+    Raw8<GT> raw[kGroup];
+    Raw8<TT> old[kGroup];
+#pragma unroll
+    for (int i = 0; i < kGroup; i++) {
+      if (ours[i]) raw[i] = loadGradient<GT>(a, (uint32_t)__builtin_amdgcn_readlane((int)mine, i), cols);
+      if (ADD && begins[i]) old[i] = loadColumns<TT>(a.table + (size_t)key[i] * a.tableStride, cols);
+    }
+    float acc[kVec] = {};
+    Raw8<TT> was{};
+#pragma unroll
+    for (int i = 0; i < kGroup; i++) {
+      if (!ours[i]) continue;
+      float f[kVec];
+      widen8<GT>(raw[i], f);
+      if (begins[i]) {
+        if constexpr (ADD) was = old[i];
+#pragma unroll
+        for (int j = 0; j < kVec; j++) acc[j] = f[j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < kVec; j++) acc[j] += f[j];
+      }
+      if (key[i + 1] == key[i]) {
+        if (i < kGroup - 1) continue;
+        // The group's last run goes on. It began at `pos`, its end is in sight unless it is long.
+        uint32_t pos = p0;
+#pragma unroll
+        for (int k = 1; k < kGroup; k++)
+          if (begins[k]) pos = p0 + k;
+        const uint64_t same = __ballot(window == key[i]) >> 1;  // bit b: position p0 + b
+        const uint64_t on = ~(same >> kGroup);                  // (bits 63 - kGroup and up are out of sight: set)
+        uint32_t end = p0 + kGroup + (uint32_t)__builtin_ctzll(on);
+        if (end == p0 + 63) end = endOfRun(keys, key[i], end, a.n, lane);
+        const uint32_t c0 = (pos + kChunk - 1) / kChunk, c1 = end / kChunk;
+        if (!a.chunked || c0 >= c1) {  // (then it ends within the 64 positions whose payloads are here)
+          addTokens<GT, 8>(a, mine, kGroup, (int)(end - p0) - kGroup, cols, acc);
+        } else {
+          const uint64_t behind = (uint64_t)c1 * kChunk + (uint32_t)lane;
+          const uint32_t rest = behind < end ? pays[behind] : 0;
+          if (c0 * kChunk == pos) {  // the chunk's sum has the group's tokens, too
+#pragma unroll
+            for (int j = 0; j < kVec; j++) acc[j] = 0.0f;
+          } else {
+            addTokens<GT, 8>(a, mine, kGroup, (int)(c0 * kChunk - p0) - kGroup, cols, acc);
+          }
+          const uint32_t s0 = (c0 + kChunk - 1) / kChunk, s1 = c1 / kChunk;
+          if (!a.supered || s0 >= s1) {
+            addSums(a.chunkSums, a.widthPad, c0, c1, cols.slot, acc);
+          } else {
+            addSums(a.chunkSums, a.widthPad, c0, s0 * kChunk, cols.slot, acc);
+            addSums(a.superSums, a.widthPad, s0, s1, cols.slot, acc);
+            addSums(a.chunkSums, a.widthPad, s1 * kChunk, c1, cols.slot, acc);
+          }
+          addTokens<GT, 8>(a, rest, 0, (int)(end - c1 * kChunk), cols, acc);
+        }
+      }
+      char* to = a.table + (size_t)key[i] * a.tableStride + (size_t)cols.at * typeSize(TT);
+      float sum[kVec];
+      if constexpr (ADD) widen8<TT>(was, sum);
+#pragma unroll
+      for (int j = 0; j < kVec; j++) sum[j] = ADD ? sum[j] + acc[j] * a.scale : acc[j] * a.scale;
+      if (cols.count == kVec && cols.shift == 0) {
+        store8<TT>(to, sum);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kVec; j++)
+          if (j >= cols.shift && j < cols.count) storeElem<typeSize(TT)>(to, j, narrow<TT>(sum[j]));
+      }
+    }
   }
 }
 
@@ -646,17 +718,20 @@ static SortKernel pickSort(bool scatter, bool longTiles, bool first) {
   if (longTiles) return first ? pickSortS<kLongStrips, true>(scatter) : pickSortS<kLongStrips, false>(scatter);
   return first ? pickSortS<kShortStrips, true>(scatter) : pickSortS<kShortStrips, false>(scatter);
 }
-typedef void (*ChunkKernel)(GradArgs, int, Clear);
 typedef void (*RowsKernel)(GradArgs, int);
-static ChunkKernel pickChunk(int gt) {
+static RowsKernel pickChunk(int gt) {
   return gt == kF32 ? chunkKernel<kF32> : gt == kF16 ? chunkKernel<kF16> : chunkKernel<kBF16>;
 }
-template <int GT>
+template <int GT, bool ADD>
 static RowsKernel pickRowsT(int tt) {
-  return tt == kF32 ? rowsKernel<GT, kF32> : tt == kF16 ? rowsKernel<GT, kF16> : rowsKernel<GT, kBF16>;
+  return tt == kF32 ? rowsKernel<GT, kF32, ADD> : tt == kF16 ? rowsKernel<GT, kF16, ADD> : rowsKernel<GT, kBF16, ADD>;
 }
-static RowsKernel pickRows(int gt, int tt) {
-  return gt == kF32 ? pickRowsT<kF32>(tt) : gt == kF16 ? pickRowsT<kF16>(tt) : pickRowsT<kBF16>(tt);
+template <bool ADD>
+static RowsKernel pickRowsG(int gt, int tt) {
+  return gt == kF32 ? pickRowsT<kF32, ADD>(tt) : gt == kF16 ? pickRowsT<kF16, ADD>(tt) : pickRowsT<kBF16, ADD>(tt);
+}
+static RowsKernel pickRows(int gt, int tt, bool accumulate) {
+  return accumulate ? pickRowsG<true>(gt, tt) : pickRowsG<false>(gt, tt);
 }
 
 // Plan of a gradient call from its sizes: how it is sorted and where the workspace's parts begin.
@@ -806,49 +881,54 @@ DFCCL_API ncclResult_t dfcclEmbeddingGrad(const void* const* grads, const void* 
   a.superSums = (float*)(ws + p.superSums);
   a.widthPad = (uint32_t)((width + kVec - 1) / kVec * kVec);
 
-  // the table's clearing, in equal shares over the launches before the rows' sums
-  const int launches = (p.small ? 1 : 2 * p.passes) + (p.chunked ? 1 : 0);
+  // the table's clearing, in equal shares over the launches of the sort
+  const uint32_t sortWaves = p.small ? kSmallWaves : kSortWaves;
+  const int launches = p.small ? 1 : 2 * p.passes;
   Clear clear{};
   uint64_t clearParts = 0;
   if (!accumulate) {
     const size_t rowBytes = width * typeSize((int)tableType);
-    const bool oneRow = a.tableStride == rowBytes;
     clear.at = a.table;
-    clear.stride = a.tableStride;
-    clear.bytes = oneRow ? (uint64_t)rowBytes * rows : rowBytes;
-    clear.parts = (clear.bytes + kClearBytes - 1) / kClearBytes;
-    clearParts = clear.parts * (oneRow ? 1 : rows);
+    if (a.tableStride == rowBytes) {
+      clear.bytes = (uint64_t)rowBytes * rows;
+      clearParts = (clear.bytes + clearPart(sortWaves) - 1) / clearPart(sortWaves);
+    } else {
+      clear.stride = a.tableStride;
+      clear.bytes = rowBytes;
+      clear.rowParts = (rowBytes + kGapBytes - 1) / kGapBytes;
+      clearParts = clear.rowParts * rows;
+    }
   }
   int launch = 0;
   // the share of the next launch, whose own work takes `blocks` workgroups; returns the launch's grid
-  auto share = [&](unsigned blocks, unsigned waves) {
+  auto share = [&](unsigned blocks) {
     clear.begin = clearParts * launch / launches;
     clear.end = clearParts * (launch + 1) / launches;
     clear.firstBlock = blocks;
     launch++;
-    const uint64_t want = (clear.end - clear.begin + waves - 1) / waves;
-    return blocks + (unsigned)std::min<uint64_t>(want, 256u * kClearWavesPerCu / waves);
+    const uint64_t parts = clear.end - clear.begin, want = clear.stride == 0 ? parts : (parts + sortWaves - 1) / sortWaves;
+    return blocks + (unsigned)std::min<uint64_t>(want, p.small ? 256 : kMaxGrid);
   };
   const hipStream_t st = (hipStream_t)stream;
   int from = 0;
   if (p.small) {
-    const unsigned grid = share(1, kSmallWaves);
+    const unsigned grid = share(1);
     DFCCL_LAUNCH_BLOCKS((n <= kSmallThreads * kFewStrips ? sortSmallKernel<kFewStrips> : sortSmallKernel<kManyStrips>), grid,
                         kSmallThreads, st, a, p.keyBits, clear);
   }
   for (int pass = 0; !p.small && pass < p.passes; pass++, from ^= 1) {
     const SortPass s{from, pass * p.digitBits, p.digitBits, p.tiles};
     for (int scatter = 0; scatter < 2; scatter++) {
-      const unsigned grid = share((unsigned)p.tiles, kSortWaves);
+      const unsigned grid = share((unsigned)p.tiles);
       DFCCL_LAUNCH_BLOCKS(pickSort(scatter != 0, p.longTiles, pass == 0), grid, kSortThreads, st, a, s, clear);
     }
   }
-  if (p.chunked) {
-    const unsigned grid = share(gridFor(n / kChunk * a.pieces), kRowWaves);
-    DFCCL_LAUNCH_BLOCKS(pickChunk((int)gradType), grid, kRowThreads, st, a, from, clear);
-  }
+  if (p.chunked)
+    DFCCL_LAUNCH_BLOCKS(pickChunk((int)gradType), gridFor(n / kChunk * a.pieces), kRowThreads, st, a, from);
   if (p.supered)
     DFCCL_LAUNCH_BLOCKS(superKernel, gridFor(n / (kChunk * kChunk) * a.pieces), kRowThreads, st, a, from);
-  if (n > 0) DFCCL_LAUNCH_BLOCKS(pickRows((int)gradType, (int)tableType), gridFor(n * a.pieces), kRowThreads, st, a, from);
+  if (n > 0)
+    DFCCL_LAUNCH_BLOCKS(pickRows((int)gradType, (int)tableType, accumulate != 0),
+                        gridFor((n + kGroup - 1) / kGroup * a.pieces), kRowThreads, st, a, from);
   return hipGetLastError() == hipSuccess ? ncclSuccess : ncclUnhandledCudaError;
 }
