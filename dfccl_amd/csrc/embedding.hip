@@ -115,7 +115,7 @@ static LookupKernel pickLookup(int in, int out) {
 //    payload, its source and number. A radix sort from the low digit up, stable and without atomics on positions,
 //    puts equal keys side by side in the order source, token: the order of every sum is fixed by the ids alone.
 // 2. Chunks. The sorted list is cut into chunks of kChunk. A chunk that lies within one row's run is summed by a
-//    wave of its own into fp32 scratch, and so are kChunk such chunks: a row that many tokens share (padding that
+//    wave of its own into fp32 scratch, and so are kSuper such chunks: a row that many tokens share (padding that
 //    counts, frequent words) is summed by many waves, and again in a fixed order.
 // 3. Rows. A wave per group of sorted positions and row piece sums the runs that begin in its group: single tokens up to
 //    the first whole chunk, whole chunks' (and chunks of chunks') sums, single tokens after the last.
@@ -123,7 +123,9 @@ static LookupKernel pickLookup(int in, int out) {
 // bytes, and it needs nothing of the sort: all rows are cleared by additional workgroups of the launches of 1.,
 // which leave most of the chip idle, and the named rows are written over afterwards.
 
-constexpr int kChunk = 32;
+constexpr int kChunk = 16;         // tokens
+constexpr int kSuper = 16;         // chunks
+constexpr int kSuperTokens = kChunk * kSuper;
 constexpr int kMaxDigitBits = 10;
 constexpr int kMaxBins = 1 << kMaxDigitBits;
 constexpr int kSrcShift = 28;  // payload: source << 28 | token, so a source has fewer than 2^28 tokens
@@ -145,7 +147,7 @@ struct GradArgs {
   uint32_t* pays[2];
   uint32_t* hist;     // [tiles][bins]
   float* chunkSums;   // [n / kChunk][widthPad]
-  float* superSums;   // [n / kChunk^2][widthPad]
+  float* superSums;   // [n / kSuperTokens][widthPad]
   uint32_t widthPad;  // width rounded up to kVec
 };
 
@@ -266,7 +268,7 @@ constexpr int kFewStrips = 4, kManyStrips = 16;
 #define DFCCL_SORT_SMALL_MAX (kSmallThreads * kManyStrips)
 #endif
 #ifndef DFCCL_SUPER_MIN
-#define DFCCL_SUPER_MIN (256 * kChunk)
+#define DFCCL_SUPER_MIN 8192
 #endif
 constexpr uint32_t kSmallMax = DFCCL_SORT_SMALL_MAX, kSuperMin = DFCCL_SUPER_MIN;
 static_assert(kSmallMax <= kSmallThreads * kManyStrips, "one workgroup sorts no more");
@@ -471,26 +473,33 @@ __global__ __launch_bounds__(kSortThreads) void sortScatterKernel(GradArgs a, So
 
 // ---- sums
 
-// A lane's eight columns of a row of a.width elements. The last lane's would reach beyond the row's end unless the width
-// is a multiple of eight: it takes the row's last eight elements instead, `shift` of which are the lane's before, and
-// only stores its own. A row of fewer than eight elements is put together from them.
+// A lane's eight columns of a row. Where they would reach beyond the row's end the lane loads the row's last eight
+// elements instead and stores only its own of them: every lane's loads are the same single instruction, none is under
+// a condition, and so all of them can be in flight. Rows of fewer than eight elements (NARROW) are put together from
+// elements.
 struct Columns {
   uint32_t at, slot;  // first column that is loaded; place in fp32 scratch (which has whole vectors)
-  int count, shift;   // elements there (8, fewer in a narrow row, 0 beyond the row); how many of them are not the lane's
+  int count, shift;   // elements of a narrow row; how many of the eight are not the lane's (8: none is)
 };
+template <bool NARROW>
 __device__ __forceinline__ Columns columnsOf(uint32_t width, uint32_t piece, int lane) {
   Columns c;
   c.slot = piece * kPieceElems + (uint32_t)lane * kVec;
-  const int left = (int)width - (int)c.slot;
-  c.shift = left > 0 && left < kVec && width >= kVec ? kVec - left : 0;
-  c.at = c.slot - (uint32_t)c.shift;
-  c.count = left <= 0 ? 0 : left + c.shift < kVec ? left + c.shift : kVec;
+  if constexpr (NARROW) {
+    c.at = 0;
+    c.count = c.slot == 0 ? (int)width : 0;
+    c.shift = c.slot == 0 ? 0 : kVec;
+  } else {
+    c.at = c.slot < width - kVec ? c.slot : width - kVec;
+    c.count = kVec;
+    c.shift = c.slot - c.at < (uint32_t)kVec ? (int)(c.slot - c.at) : kVec;
+  }
   return c;
 }
-template <int DT>
+template <int DT, bool NARROW>
 __device__ __forceinline__ Raw8<DT> loadColumns(const char* row, const Columns& c) {
   const char* p = row + (size_t)c.at * typeSize(DT);
-  if (c.count == kVec) return loadRaw8<DT>(p);
+  if constexpr (!NARROW) return loadRaw8<DT>(p);
   Raw8<DT> r{};
 #pragma unroll 1
   for (int j = c.count - 1; j >= 0; j--) {  // (in from the low end)
@@ -506,41 +515,72 @@ __device__ __forceinline__ Raw8<DT> loadColumns(const char* row, const Columns& 
   }
   return r;
 }
-template <int GT>
-__device__ __forceinline__ Raw8<GT> loadGradient(const GradArgs& a, uint32_t pay, const Columns& c) {
-  return loadColumns<GT>(a.grads[pay >> kSrcShift] + (size_t)(pay & kTokenMask) * a.gradStride, c);
-}
-
-// acc += the gradients of `count` tokens whose payloads lanes from .. from + count - 1 hold, this lane's eight columns,
-// in order. The payloads come by lane, so the loads depend on nothing but each other's registers: AHEAD are in flight.
-template <int GT, int AHEAD>
-__device__ __forceinline__ void addTokens(const GradArgs& a, uint32_t pays, int from, int count, const Columns& c,
-                                          float (&acc)[kVec]) {
-  for (int p = 0; p < count; p += AHEAD) {
-    Raw8<GT> raw[AHEAD];
+template <int DT, bool NARROW>
+__device__ __forceinline__ void storeColumns(char* row, const Columns& c, const Raw8<DT>& r) {
+  char* p = row + (size_t)c.at * typeSize(DT);
+  if (!NARROW && c.shift == 0) {
+    store16<typeSize(DT)>(p, r.w[0]);
+    if constexpr (DT == kF32) store16<4>(p + 16, r.w[1]);
+  } else if (c.shift < kVec) {
 #pragma unroll
-    for (int i = 0; i < AHEAD; i++)
-      if (p + i < count) raw[i] = loadGradient<GT>(a, (uint32_t)__builtin_amdgcn_readlane((int)pays, from + p + i), c);
-#pragma unroll
-    for (int i = 0; i < AHEAD; i++)
-      if (p + i < count) {
-        float f[kVec];
-        widen8<GT>(raw[i], f);
-#pragma unroll
-        for (int j = 0; j < kVec; j++) acc[j] += f[j];
+    for (int j = 0; j < kVec; j++)
+      if (j >= c.shift && j < c.count) {
+        if constexpr (DT == kF32) storeElem<4>(p, j, r.w[j / 4][j % 4]);
+        else storeElem<2>(p, j, (r.w[0][j / 2] >> (16 * (j % 2))) & 0xffffu);
       }
   }
 }
+// Where the gradient rows of the tokens are whose payloads the lanes hold. A lane picks its source's pointer out of the
+// kernel's arguments for itself, and the wave takes a token's address from its lane: a load of the pointer, scalar or
+// not, would have to be waited for before the row's.
+struct TokenRows {
+  uint32_t lo, hi;
+};
+__device__ __forceinline__ TokenRows rowsOf(const GradArgs& a, uint32_t pay) {
+  const char* base = a.grads[0];
+#pragma unroll
+  for (uint32_t r = 1; r < kMaxSrcs; r++) base = (pay >> kSrcShift) == r ? a.grads[r] : base;
+  const uint64_t at = (uint64_t)(uintptr_t)base + (uint64_t)(pay & kTokenMask) * a.gradStride;
+  return TokenRows{(uint32_t)at, (uint32_t)(at >> 32)};
+}
+__device__ __forceinline__ const char* rowOfLane(const TokenRows& r, int lane) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)r.lo, lane), hi = (uint32_t)__builtin_amdgcn_readlane((int)r.hi, lane);
+  return (const char*)(uintptr_t)(((uint64_t)hi << 32) | lo);
+}
+
+// acc += the gradients of the `count` tokens whose rows lanes from .. from + count - 1 hold, this lane's eight columns, in
+// order. None of the loads is under a condition (the last few, less than AHEAD, repeat the last token's), or the compiler
+// would wait for each by itself.
+template <int GT, bool NARROW, int AHEAD>
+__device__ __forceinline__ void addBatch(const TokenRows& rows, int from, int count, const Columns& c, float (&acc)[kVec]) {
+  Raw8<GT> raw[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; i++) raw[i] = loadColumns<GT, NARROW>(rowOfLane(rows, from + (i < count ? i : count - 1)), c);
+#pragma unroll
+  for (int i = 0; i < AHEAD; i++)
+    if (i < count) {
+      float f[kVec];
+      widen8<GT>(raw[i], f);
+#pragma unroll
+      for (int j = 0; j < kVec; j++) acc[j] += f[j];
+    }
+}
+template <int GT, bool NARROW, int AHEAD>
+__device__ __forceinline__ void addTokens(const TokenRows& rows, int from, int count, const Columns& c, float (&acc)[kVec]) {
+  int p = 0;
+  for (; p + AHEAD <= count; p += AHEAD) addBatch<GT, NARROW, AHEAD>(rows, from + p, AHEAD, c, acc);
+  for (; p < count; p += 4) addBatch<GT, NARROW, 4>(rows, from + p, count - p < 4 ? count - p : 4, c, acc);
+}
 // acc += rows [begin, end) of fp32 scratch
-__device__ __forceinline__ void addSums(const float* sums, uint32_t widthPad, uint32_t begin, uint32_t end, uint32_t col,
+__device__ __forceinline__ void addSums(const float* sums, uint32_t widthPad, uint32_t begin, uint32_t end, uint32_t slot,
                                         float (&acc)[kVec]) {
-  if (col >= widthPad) return;
+  if (slot >= widthPad) return;
   constexpr int kAhead = 8;
   for (uint32_t c = begin; c < end; c += kAhead) {
     Raw8<kF32> raw[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; i++)
-      if (c + i < end) raw[i] = loadRaw8<kF32>((const char*)(sums + (size_t)(c + i) * widthPad + col));
+      raw[i] = loadRaw8<kF32>((const char*)(sums + (size_t)(c + i < end ? c + i : end - 1) * widthPad + slot));
 #pragma unroll
     for (int i = 0; i < kAhead; i++)
       if (c + i < end) {
@@ -552,8 +592,12 @@ __device__ __forceinline__ void addSums(const float* sums, uint32_t widthPad, ui
   }
 }
 
-// One wave per (chunk, piece): the chunk's sum if all of it belongs to one row.
+// (twice as many take the registers of two waves per SIMD and gain nothing)
 template <int GT>
+constexpr int kTokensAhead = GT == kF32 ? 4 : 8;
+
+// One wave per (chunk, piece): the chunk's sum if all of it belongs to one row.
+template <int GT, bool NARROW>
 __global__ __launch_bounds__(kRowThreads) void chunkKernel(GradArgs a, int sorted) {
   const int lane = (int)(threadIdx.x & 63);
   const uint32_t* keys = a.keys[sorted];
@@ -561,29 +605,34 @@ __global__ __launch_bounds__(kRowThreads) void chunkKernel(GradArgs a, int sorte
   for (uint64_t item = (uint64_t)blockIdx.x * kRowWaves + waveInBlock(); item < items;
        item += (uint64_t)gridDim.x * kRowWaves) {
     const uint32_t chunk = (uint32_t)(item / a.pieces), piece = (uint32_t)(item % a.pieces), begin = chunk * kChunk;
-    const uint32_t first = keys[begin], last = keys[begin + kChunk - 1], pays = a.pays[sorted][begin + (lane & (kChunk - 1))];
-    const uint32_t key = uniform(first);
-    if (key >= a.rows || uniform(last) != key) continue;
-    const Columns cols = columnsOf(a.width, piece, lane);
+    uint32_t mine = keys[begin + (lane & (kChunk - 1))], pays = a.pays[sorted][begin + (lane & (kChunk - 1))];
+    DFCCL_LOADED(mine);
+    DFCCL_LOADED(pays);
+    const uint32_t key = (uint32_t)__builtin_amdgcn_readlane((int)mine, 0);
+    const uint32_t last = (uint32_t)__builtin_amdgcn_readlane((int)mine, kChunk - 1);
+    if (key >= a.rows || last != key) continue;
+    const Columns cols = columnsOf<NARROW>(a.width, piece, lane);
     float acc[kVec] = {};
-    addTokens<GT, GT == kF32 ? 8 : 16>(a, pays, 0, kChunk, cols, acc);
-    if (cols.count > 0) store8<kF32>((char*)(a.chunkSums + (size_t)chunk * a.widthPad + cols.slot), acc);
+    addTokens<GT, NARROW, kTokensAhead<GT>>(rowsOf(a, pays), 0, kChunk, cols, acc);
+    if (cols.shift < kVec) store8<kF32>((char*)(a.chunkSums + (size_t)chunk * a.widthPad + cols.slot), acc);
   }
 }
 // One wave per (chunk of chunks, piece)
 __global__ __launch_bounds__(kRowThreads) void superKernel(GradArgs a, int sorted) {
   const int lane = (int)(threadIdx.x & 63);
   const uint32_t* keys = a.keys[sorted];
-  const uint64_t items = (uint64_t)(a.n / (kChunk * kChunk)) * a.pieces;
+  const uint64_t items = (uint64_t)(a.n / kSuperTokens) * a.pieces;
   for (uint64_t item = (uint64_t)blockIdx.x * kRowWaves + waveInBlock(); item < items;
        item += (uint64_t)gridDim.x * kRowWaves) {
     const uint32_t super = (uint32_t)(item / a.pieces), piece = (uint32_t)(item % a.pieces);
-    const uint32_t begin = super * (kChunk * kChunk), first = keys[begin], last = keys[begin + kChunk * kChunk - 1];
+    uint32_t first = keys[super * kSuperTokens], last = keys[super * kSuperTokens + kSuperTokens - 1];
+    DFCCL_LOADED(first);
+    DFCCL_LOADED(last);
     const uint32_t key = uniform(first);
     if (key >= a.rows || uniform(last) != key) continue;
     const uint32_t col = piece * kPieceElems + lane * kVec;
     float acc[kVec] = {};
-    addSums(a.chunkSums, a.widthPad, super * kChunk, (super + 1) * kChunk, col, acc);
+    addSums(a.chunkSums, a.widthPad, super * kSuper, (super + 1) * kSuper, col, acc);
     if (col < a.widthPad) store8<kF32>((char*)(a.superSums + (size_t)super * a.widthPad + col), acc);
   }
 }
@@ -610,7 +659,7 @@ __device__ __forceinline__ uint32_t endOfRun(const uint32_t* keys, uint32_t key,
 constexpr int kGroup = 4;
 static_assert(kChunk % kGroup == 0, "a group lies within one chunk");
 
-template <int GT, int TT, bool ADD>
+template <int GT, int TT, bool ADD, bool NARROW>
 __global__ __launch_bounds__(kRowThreads) void rowsKernel(GradArgs a, int sorted) {
   const int lane = (int)(threadIdx.x & 63);
   const uint32_t *keys = a.keys[sorted], *pays = a.pays[sorted];
@@ -618,11 +667,13 @@ __global__ __launch_bounds__(kRowThreads) void rowsKernel(GradArgs a, int sorted
   for (uint64_t item = (uint64_t)blockIdx.x * kRowWaves + waveInBlock(); item < items;
        item += (uint64_t)gridDim.x * kRowWaves) {
     const uint64_t group = item / a.pieces;
-    const Columns cols = columnsOf(a.width, (uint32_t)(item - group * a.pieces), lane);
+    const Columns cols = columnsOf<NARROW>(a.width, (uint32_t)(item - group * a.pieces), lane);
     const uint32_t p0 = (uint32_t)group * kGroup;
     const uint64_t at = (uint64_t)p0 + (uint32_t)lane;
-    const uint32_t window = at >= 1 && at - 1 < a.n ? keys[at - 1] : a.rows;  // lane l: position p0 - 1 + l
-    const uint32_t mine = at < a.n ? pays[at] : 0;                            // lane l: position p0 + l
+    uint32_t window = at >= 1 && at - 1 < a.n ? keys[at - 1] : a.rows;  // lane l: position p0 - 1 + l
+    uint32_t mine = at < a.n ? pays[at] : 0;                            // lane l: position p0 + l
+    DFCCL_LOADED(window);
+    DFCCL_LOADED(mine);
     uint32_t key[kGroup + 1];
     bool begins[kGroup], ours[kGroup];  // ours: of a run that begins in the group
     uint32_t before = (uint32_t)__builtin_amdgcn_readlane((int)window, 0);
@@ -637,30 +688,42 @@ __global__ __launch_bounds__(kRowThreads) void rowsKernel(GradArgs a, int sorted
       before = key[i];
     }
     if (!any) continue;
+    // Positions that are not ours load what the first one that begins a run does (nothing is under a condition: see
+    // addBatch), and every sum is complete before the first is stored: loads and stores are counted together, and a
+    // wait for a load behind a store is one for the store.
+    int some = 0;
+    uint32_t someKey = 0;
+#pragma unroll
+    for (int i = kGroup - 1; i >= 0; i--)
+      if (begins[i]) {
+        some = i;
+        someKey = key[i];
+      }
+    const TokenRows tokens = rowsOf(a, mine);
     Raw8<GT> raw[kGroup];
-    Raw8<TT> old[kGroup];
+    Raw8<TT> old[kGroup], out[kGroup];
 #pragma unroll
-    for (int i = 0; i < kGroup; i++) {
-      if (ours[i]) raw[i] = loadGradient<GT>(a, (uint32_t)__builtin_amdgcn_readlane((int)mine, i), cols);
-      if (ADD && begins[i]) old[i] = loadColumns<TT>(a.table + (size_t)key[i] * a.tableStride, cols);
+    for (int i = 0; i < kGroup; i++) raw[i] = loadColumns<GT, NARROW>(rowOfLane(tokens, ours[i] ? i : some), cols);
+    if constexpr (ADD) {
+#pragma unroll
+      for (int i = 0; i < kGroup; i++)
+        old[i] = loadColumns<TT, NARROW>(a.table + (size_t)(begins[i] ? key[i] : someKey) * a.tableStride, cols);
     }
-    float acc[kVec] = {};
-    Raw8<TT> was{};
+    float acc[kVec] = {}, was[kVec] = {};
+    bool ends[kGroup];
 #pragma unroll
     for (int i = 0; i < kGroup; i++) {
-      if (!ours[i]) continue;
       float f[kVec];
       widen8<GT>(raw[i], f);
-      if (begins[i]) {
-        if constexpr (ADD) was = old[i];
 #pragma unroll
-        for (int j = 0; j < kVec; j++) acc[j] = f[j];
-      } else {
+      for (int j = 0; j < kVec; j++) acc[j] = begins[i] ? f[j] : acc[j] + f[j];
+      if constexpr (ADD) {
+        widen8<TT>(old[i], f);
 #pragma unroll
-        for (int j = 0; j < kVec; j++) acc[j] += f[j];
+        for (int j = 0; j < kVec; j++) was[j] = begins[i] ? f[j] : was[j];
       }
-      if (key[i + 1] == key[i]) {
-        if (i < kGroup - 1) continue;
+      ends[i] = ours[i] && (i == kGroup - 1 || key[i + 1] != key[i]);
+      if (i == kGroup - 1 && ours[i] && key[i + 1] == key[i]) {
         // The group's last run goes on. It began at `pos`, its end is in sight unless it is long.
         uint32_t pos = p0;
 #pragma unroll
@@ -672,7 +735,7 @@ __global__ __launch_bounds__(kRowThreads) void rowsKernel(GradArgs a, int sorted
         if (end == p0 + 63) end = endOfRun(keys, key[i], end, a.n, lane);
         const uint32_t c0 = (pos + kChunk - 1) / kChunk, c1 = end / kChunk;
         if (!a.chunked || c0 >= c1) {  // (then it ends within the 64 positions whose payloads are here)
-          addTokens<GT, 8>(a, mine, kGroup, (int)(end - p0) - kGroup, cols, acc);
+          addTokens<GT, NARROW, kTokensAhead<GT>>(tokens, kGroup, (int)(end - p0) - kGroup, cols, acc);
         } else {
           const uint64_t behind = (uint64_t)c1 * kChunk + (uint32_t)lane;
           const uint32_t rest = behind < end ? pays[behind] : 0;
@@ -680,32 +743,27 @@ __global__ __launch_bounds__(kRowThreads) void rowsKernel(GradArgs a, int sorted
 #pragma unroll
             for (int j = 0; j < kVec; j++) acc[j] = 0.0f;
           } else {
-            addTokens<GT, 8>(a, mine, kGroup, (int)(c0 * kChunk - p0) - kGroup, cols, acc);
+            addTokens<GT, NARROW, kTokensAhead<GT>>(tokens, kGroup, (int)(c0 * kChunk - p0) - kGroup, cols, acc);
           }
-          const uint32_t s0 = (c0 + kChunk - 1) / kChunk, s1 = c1 / kChunk;
+          const uint32_t s0 = (c0 + kSuper - 1) / kSuper, s1 = c1 / kSuper;
           if (!a.supered || s0 >= s1) {
             addSums(a.chunkSums, a.widthPad, c0, c1, cols.slot, acc);
           } else {
-            addSums(a.chunkSums, a.widthPad, c0, s0 * kChunk, cols.slot, acc);
+            addSums(a.chunkSums, a.widthPad, c0, s0 * kSuper, cols.slot, acc);
             addSums(a.superSums, a.widthPad, s0, s1, cols.slot, acc);
-            addSums(a.chunkSums, a.widthPad, s1 * kChunk, c1, cols.slot, acc);
+            addSums(a.chunkSums, a.widthPad, s1 * kSuper, c1, cols.slot, acc);
           }
-          addTokens<GT, 8>(a, rest, 0, (int)(end - c1 * kChunk), cols, acc);
+          addTokens<GT, NARROW, kTokensAhead<GT>>(rowsOf(a, rest), 0, (int)(end - c1 * kChunk), cols, acc);
         }
       }
-      char* to = a.table + (size_t)key[i] * a.tableStride + (size_t)cols.at * typeSize(TT);
       float sum[kVec];
-      if constexpr (ADD) widen8<TT>(was, sum);
 #pragma unroll
-      for (int j = 0; j < kVec; j++) sum[j] = ADD ? sum[j] + acc[j] * a.scale : acc[j] * a.scale;
-      if (cols.count == kVec && cols.shift == 0) {
-        store8<TT>(to, sum);
-      } else {
-#pragma unroll
-        for (int j = 0; j < kVec; j++)
-          if (j >= cols.shift && j < cols.count) storeElem<typeSize(TT)>(to, j, narrow<TT>(sum[j]));
-      }
+      for (int j = 0; j < kVec; j++) sum[j] = ADD ? was[j] + acc[j] * a.scale : acc[j] * a.scale;
+      out[i] = narrow8<TT>(sum);
     }
+#pragma unroll
+    for (int i = 0; i < kGroup; i++)
+      if (ends[i]) storeColumns<TT, NARROW>(a.table + (size_t)key[i] * a.tableStride, cols, out[i]);
   }
 }
 
@@ -719,19 +777,26 @@ static SortKernel pickSort(bool scatter, bool longTiles, bool first) {
   return first ? pickSortS<kShortStrips, true>(scatter) : pickSortS<kShortStrips, false>(scatter);
 }
 typedef void (*RowsKernel)(GradArgs, int);
-static RowsKernel pickChunk(int gt) {
-  return gt == kF32 ? chunkKernel<kF32> : gt == kF16 ? chunkKernel<kF16> : chunkKernel<kBF16>;
+template <bool NARROW>
+static RowsKernel pickChunkN(int gt) {
+  return gt == kF32 ? chunkKernel<kF32, NARROW> : gt == kF16 ? chunkKernel<kF16, NARROW> : chunkKernel<kBF16, NARROW>;
 }
-template <int GT, bool ADD>
+static RowsKernel pickChunk(int gt, bool narrow) { return narrow ? pickChunkN<true>(gt) : pickChunkN<false>(gt); }
+template <int GT, bool ADD, bool NARROW>
 static RowsKernel pickRowsT(int tt) {
-  return tt == kF32 ? rowsKernel<GT, kF32, ADD> : tt == kF16 ? rowsKernel<GT, kF16, ADD> : rowsKernel<GT, kBF16, ADD>;
+  return tt == kF32   ? rowsKernel<GT, kF32, ADD, NARROW>
+         : tt == kF16 ? rowsKernel<GT, kF16, ADD, NARROW>
+                      : rowsKernel<GT, kBF16, ADD, NARROW>;
 }
-template <bool ADD>
+template <bool ADD, bool NARROW>
 static RowsKernel pickRowsG(int gt, int tt) {
-  return gt == kF32 ? pickRowsT<kF32, ADD>(tt) : gt == kF16 ? pickRowsT<kF16, ADD>(tt) : pickRowsT<kBF16, ADD>(tt);
+  return gt == kF32   ? pickRowsT<kF32, ADD, NARROW>(tt)
+         : gt == kF16 ? pickRowsT<kF16, ADD, NARROW>(tt)
+                      : pickRowsT<kBF16, ADD, NARROW>(tt);
 }
-static RowsKernel pickRows(int gt, int tt, bool accumulate) {
-  return accumulate ? pickRowsG<true>(gt, tt) : pickRowsG<false>(gt, tt);
+static RowsKernel pickRows(int gt, int tt, bool accumulate, bool narrow) {
+  if (narrow) return accumulate ? pickRowsG<true, true>(gt, tt) : pickRowsG<false, true>(gt, tt);
+  return accumulate ? pickRowsG<true, false>(gt, tt) : pickRowsG<false, false>(gt, tt);
 }
 
 // Plan of a gradient call from its sizes: how it is sorted and where the workspace's parts begin.
@@ -767,7 +832,7 @@ static GradPlan planGrad(uint64_t n, size_t rows, size_t width) {
   }
   if (!p.small) p.hist = take(((size_t)p.tiles << p.digitBits) * 4);
   if (p.chunked) p.chunkSums = take(n / kChunk * widthPad * 4);
-  if (p.supered) p.superSums = take(n / (kChunk * kChunk) * widthPad * 4);
+  if (p.supered) p.superSums = take(n / kSuperTokens * widthPad * 4);
   p.bytes = std::max<size_t>(at, 256);
   return p;
 }
@@ -882,6 +947,7 @@ DFCCL_API ncclResult_t dfcclEmbeddingGrad(const void* const* grads, const void* 
   a.widthPad = (uint32_t)((width + kVec - 1) / kVec * kVec);
 
   // the table's clearing, in equal shares over the launches of the sort
+  const bool narrow = width < kVec;
   const uint32_t sortWaves = p.small ? kSmallWaves : kSortWaves;
   const int launches = p.small ? 1 : 2 * p.passes;
   Clear clear{};
@@ -924,11 +990,11 @@ DFCCL_API ncclResult_t dfcclEmbeddingGrad(const void* const* grads, const void* 
     }
   }
   if (p.chunked)
-    DFCCL_LAUNCH_BLOCKS(pickChunk((int)gradType), gridFor(n / kChunk * a.pieces), kRowThreads, st, a, from);
+    DFCCL_LAUNCH_BLOCKS(pickChunk((int)gradType, narrow), gridFor(n / kChunk * a.pieces), kRowThreads, st, a, from);
   if (p.supered)
-    DFCCL_LAUNCH_BLOCKS(superKernel, gridFor(n / (kChunk * kChunk) * a.pieces), kRowThreads, st, a, from);
+    DFCCL_LAUNCH_BLOCKS(superKernel, gridFor(n / kSuperTokens * a.pieces), kRowThreads, st, a, from);
   if (n > 0)
-    DFCCL_LAUNCH_BLOCKS(pickRows((int)gradType, (int)tableType, accumulate != 0),
+    DFCCL_LAUNCH_BLOCKS(pickRows((int)gradType, (int)tableType, accumulate != 0, narrow),
                         gridFor((n + kGroup - 1) / kGroup * a.pieces), kRowThreads, st, a, from);
   return hipGetLastError() == hipSuccess ? ncclSuccess : ncclUnhandledCudaError;
 }

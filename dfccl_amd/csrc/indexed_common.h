@@ -20,6 +20,11 @@
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront"); \
   } while (0)
 #endif
+// the value, loaded, is here from this place on: loads whose values several such statements in a row name are waited for
+// together, where the compiler would move one behind a branch that only needs the other
+#ifndef DFCCL_LOADED
+#define DFCCL_LOADED(v) asm volatile("" : "+v"(v))
+#endif
 // a launch whose workgroups do not wait for each other (the host build runs a few of them at a time)
 #ifndef DFCCL_LAUNCH_BLOCKS
 #define DFCCL_LAUNCH_BLOCKS(kernel, grid, block, stream, ...) \
@@ -133,23 +138,26 @@ __device__ __forceinline__ void widen8(const Raw8<DT>& r, float (&f)[kVec]) {
     for (int i = 0; i < 4; i++) widenWord<DT>(r.w[0][i], f[2 * i], f[2 * i + 1]);
   }
 }
-template <int DT, bool NT = false>
-__device__ __forceinline__ void store8(char* p, const float (&f)[kVec]) {
-  u32x4 a;
+template <int DT>
+__device__ __forceinline__ Raw8<DT> narrow8(const float (&f)[kVec]) {  // to nearest even
+  Raw8<DT> r;
   if constexpr (DT == kF32) {
-    u32x4 b;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      a[i] = __float_as_uint(f[i]);
-      b[i] = __float_as_uint(f[4 + i]);
+      r.w[0][i] = __float_as_uint(f[i]);
+      r.w[1][i] = __float_as_uint(f[4 + i]);
     }
-    store16<4, NT>(p, a);
-    store16<4, NT>(p + 16, b);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; i++) a[i] = narrowWord<DT>(f[2 * i], f[2 * i + 1]);
-    store16<2, NT>(p, a);
+    for (int i = 0; i < 4; i++) r.w[0][i] = narrowWord<DT>(f[2 * i], f[2 * i + 1]);
   }
+  return r;
+}
+template <int DT, bool NT = false>
+__device__ __forceinline__ void store8(char* p, const float (&f)[kVec]) {
+  const Raw8<DT> r = narrow8<DT>(f);
+  store16<typeSize(DT), NT>(p, r.w[0]);
+  if constexpr (DT == kF32) store16<4, NT>(p + 16, r.w[1]);
 }
 // the last, shorter vector of a row: `left` elements (1..7)
 template <int DT>

@@ -168,6 +168,7 @@ void launchBlocks(Stream* s, unsigned grid, unsigned block, std::function<void()
 
 #define DFCCL_WAVE_UNIFORM(x) ::emul::shflFrom((x), 0, __LINE__)
 #define DFCCL_UNIFORM(x) ::emul::uniformChecked((x), __LINE__)
+#define DFCCL_LOADED(v) ((void)0)  // (likewise)
 #define DFCCL_FRESH_PER_ROUND(v) ((void)0)  // (a hint for the GPU compiler's register allocation)
 
 // EMUL_NEVER_LEAVE=1: the daemon's workgroups ignore every reason to leave (see DFCCL_TEST_NEVER_LEAVES in daemon.hip)

@@ -178,8 +178,8 @@ def test_grad_widths_and_strides(width, accumulate):
               torch.float32, accumulate=accumulate, pad=pad)
 
 
-# runs around the block of 32 and the block of 32 blocks, at every place within a block
-@pytest.mark.parametrize("tokens", [1, 2, 31, 32, 33, 63, 64, 65, 100, 1023, 1024, 1025, 2080, 3100])
+# runs around the block of 16 tokens, the 64 that a wave sees, and the block of 16 blocks
+@pytest.mark.parametrize("tokens", [1, 2, 15, 16, 17, 31, 32, 33, 62, 63, 64, 65, 66, 100, 255, 256, 257, 1023, 1024, 1300, 3100])
 @pytest.mark.parametrize("accumulate", [False, True])
 def test_grad_of_one_token_many_times(tokens, accumulate):
     _grad([_randn(24, tokens, 24)], [torch.full((tokens,), 3, device=gpu_util.DEVICE)], 5, torch.float32,
@@ -195,9 +195,9 @@ def test_grad_of_one_token_thousands_of_times(tokens):
         _grad([_randn(24, tokens + ahead, 24)], [ids], 5, torch.float32)
 
 
-@pytest.mark.parametrize("ahead", [0, 1, 17, 32, 40])
+@pytest.mark.parametrize("ahead", [0, 1, 2, 3, 4, 13, 15, 16, 17, 31, 250])
 def test_grad_of_long_runs_that_begin_anywhere(ahead):
-    ids = torch.cat([torch.full((n,), v) for v, n in ((0, ahead), (2, 1100), (3, 1), (4, 64), (6, 2100))])
+    ids = torch.cat([torch.full((n,), v) for v, n in ((0, ahead), (2, 600), (3, 1), (4, 64), (5, 31), (6, 600))])
     ids = ids[torch.randperm(ids.numel(), generator=torch.Generator().manual_seed(ahead))].to(gpu_util.DEVICE)
     _grad([_randn(25, ids.numel(), 16, dtype=torch.float16)], [ids], 8, torch.float32, scale=-0.1)
 
