@@ -51,7 +51,10 @@ struct LookupArgs {
   float scale;
 };
 
-// One wave takes one piece (512 elements) of U tokens' rows: the U ids, then the U loads are in flight together.
+// One wave takes one piece (512 elements) of U tokens' rows: the U ids, then the U loads are in flight together. Bound by
+// HBM: 16385 rows of 4096, fp32 in, bfloat16 out, 46 us = 5.4 TB/s on each different row once (a dense copy of as much
+// takes 41 us). Two rows a wave: 46 us, four 48, one 53; stores that stay in the caches: 55 (they push the table's
+// frequent rows out). fp32 outputs are stored in two halves of a line each, which have to meet in a cache.
 template <int IN, int OUT, int U>
 __global__ __launch_bounds__(kRowThreads) void lookupKernel(LookupArgs a) {
   const int lane = (int)(threadIdx.x & 63);
@@ -140,7 +143,7 @@ struct GradArgs {
   int64_t firstRow, paddingId;
   uint32_t rows, width, pieces, n;
   float scale;
-  bool accumulate, chunked, supered;  // (whether there are sums of chunks, and of chunks of chunks)
+  bool chunked, supered;  // whether there are sums of chunks, and of chunks of chunks
   char* table;
   // workspace
   uint32_t* keys[2];
@@ -259,7 +262,10 @@ __device__ __forceinline__ uint32_t waveScan(uint32_t v, int lane) {  // inclusi
   return v;
 }
 
-// ---- up to some ten thousand tokens: sorted by one workgroup in LDS, one launch instead of two per digit
+// ---- up to 16384 tokens: sorted by one workgroup in LDS, one launch instead of two per digit. Bound by the latency of
+// its steps (per digit six barriers and a ballot per bit and 64 keys): 12 us for 3600 tokens and 14 bits, where counts
+// and scatters took 23 in four launches; 52 us for 16384 tokens and 18 bits, where those took 38, but there one launch
+// lets the table's clearing (167 us for 1 GiB) run beside it without a break: 253 instead of 282 us for the whole call.
 constexpr int kSmallThreads = 1024;
 constexpr int kSmallWaves = kSmallThreads / 64;
 constexpr int kFewStrips = 4, kManyStrips = 16;
@@ -357,7 +363,7 @@ __global__ __launch_bounds__(kSmallThreads) void sortSmallKernel(GradArgs a, int
   }
 }
 
-// ---- more tokens: tiles, a count and a scatter per digit
+// ---- more tokens: tiles, a count and a scatter per digit (5 and 15 us at 16384 tokens)
 constexpr int kSortThreads = 256;
 constexpr int kSortWaves = kSortThreads / 64;
 // strips of a tile: few enough that some ten thousand tokens spread over several workgroups, many enough that
@@ -596,7 +602,9 @@ __device__ __forceinline__ void addSums(const float* sums, uint32_t widthPad, ui
 template <int GT>
 constexpr int kTokensAhead = GT == kF32 ? 4 : 8;
 
-// One wave per (chunk, piece): the chunk's sum if all of it belongs to one row.
+// One wave per (chunk, piece): the chunk's sum if all of it belongs to one row. Chunks of 16 tokens and of 16 chunks: a run
+// then ends in at most 15 tokens, 15 chunks on either side, so the wave that joins it waits for few loads in turn (with
+// 32 and 32 the most frequent of 16384 tokens kept its wave for 20 us more).
 template <int GT, bool NARROW>
 __global__ __launch_bounds__(kRowThreads) void chunkKernel(GradArgs a, int sorted) {
   const int lane = (int)(threadIdx.x & 63);
@@ -655,7 +663,10 @@ __device__ __forceinline__ uint32_t endOfRun(const uint32_t* keys, uint32_t key,
 // One wave per (group of kGroup sorted positions, piece): the runs that begin in the group. A lane each reads the keys
 // from the one before the group on and the payloads from the group's first on, so after one load it is known where
 // runs begin and end and whom they sum; then the group's rows (and the table's, if they are added to) are in flight
-// together. Only the group's last run may go on behind it.
+// together. Only the group's last run may go on behind it. Bound by HBM where the table is large: it reads and writes
+// the rows (190 MB of them in 55 us at 16384 tokens) while the 256 MB of cleared rows that the last cache level still
+// holds are written back. Four positions a wave: 55 us, two 68; a position a wave, with the lanes' loads one after the
+// other: 71.
 constexpr int kGroup = 4;
 static_assert(kChunk % kGroup == 0, "a group lies within one chunk");
 
@@ -879,7 +890,8 @@ DFCCL_API ncclResult_t dfcclEmbeddingLookup(const void* table, ncclDataType_t ta
   a.idBytes = idType == ncclInt64 ? 8 : 4;
   a.scale = (float)scale;
   constexpr int U = 2;
-  // two rows a wave once that still fills the chip (256 CUs, 32 waves each); below, one row a wave
+  // two rows a wave once that still fills the chip (256 CUs, 32 waves each), see lookupKernel; below, one row a wave:
+  // a few rows are bound by latency, which more waves with less each hide better
   const bool many = (uint64_t)tokens * a.pieces >= (uint64_t)U * 256 * 32;
   const uint64_t waves = (uint64_t)((tokens + (many ? U : 1) - 1) / (many ? U : 1)) * a.pieces;
   LookupKernel fn = many ? pickLookup<U>((int)tableType, (int)outType) : pickLookup<1>((int)tableType, (int)outType);
@@ -938,7 +950,6 @@ DFCCL_API ncclResult_t dfcclEmbeddingGrad(const void* const* grads, const void* 
     a.keys[i] = (uint32_t*)(ws + p.keys[i]);
     a.pays[i] = (uint32_t*)(ws + p.pays[i]);
   }
-  a.accumulate = accumulate != 0;
   a.chunked = p.chunked;
   a.supered = p.supered;
   a.hist = (uint32_t*)(ws + p.hist);

@@ -50,11 +50,12 @@ template <>
 struct Pack16<4> {
   typedef u32x4 type __attribute__((aligned(4)));
 };
-template <int A>
+// NT: what is not used again soon does not stay in the caches
+template <int A, bool NT = false>
 __device__ __forceinline__ u32x4 load16(const char* p) {
-  return *(const DFCCL_GLOBAL typename Pack16<A>::type*)p;
+  if constexpr (NT) return __builtin_nontemporal_load((const DFCCL_GLOBAL typename Pack16<A>::type*)p);
+  else return *(const DFCCL_GLOBAL typename Pack16<A>::type*)p;
 }
-// NT: what is not read again soon does not stay in the caches
 template <int A, bool NT = false>
 __device__ __forceinline__ void store16(char* p, u32x4 v) {
   if constexpr (NT) __builtin_nontemporal_store(v, (DFCCL_GLOBAL typename Pack16<A>::type*)p);

@@ -26,9 +26,11 @@ constexpr int kScanThreads = DFCCL_SCAN_THREADS;
 constexpr int kScanWaves = kScanThreads / 64;
 constexpr int kScanPer = 4;  // counts a thread reads at once
 constexpr int kScanTile = kScanThreads * kScanPer;
-// Up to so many tiles one workgroup scans all pages; above, a workgroup per tile counts and another launch lists.
+// Up to so many tiles one workgroup scans all pages (5 us for 2048, 6 for 8192); above, a workgroup per tile counts and
+// another launch lists (7 + 5 us for 262144 pages, where one workgroup took 54).
 constexpr int kOneScan = 4;
-constexpr int kFewRequests = 64;  // of an extend, carried out by the one workgroup that scans: a few for each of its waves
+constexpr int kFewRequests = 64;  // of an extend, carried out by the workgroup that scans: four for each of its waves, one
+                                  // launch less (15 us for a turn of 16 sequences instead of 19)
 
 // The bookkeeping as the kernels see it.
 struct Books {
@@ -268,17 +270,19 @@ struct PoolSet {
   uint32_t lastBytes;  // of a page's last part
   size_t pageBytes;
 };
-constexpr int kPartLoads = 4;                                     // 16-byte loads a lane has in flight
-constexpr uint32_t kPartBytes = 64 * 16 * kPartLoads;             // what one wave moves at a time
+// What one wave moves at a time, in 16-byte loads a lane has in flight: the sweeps behind each figure in the kernels.
+constexpr int kCopyLoads = 1, kForkLoads = 2, kCompactLoads = 4;
+constexpr uint32_t partBytes(int loads) { return 64 * 16 * (uint32_t)loads; }
 
-// one part of a page, by one wave
+// one part of a page, by one wave; stores (and with NT loads, too) do not stay in the caches
+template <int LOADS, bool NT>
 __device__ __forceinline__ void movePart(const char* from, char* to, uint32_t bytes, uint32_t lane) {
-  if (bytes == kPartBytes) {
-    u32x4 v[kPartLoads];
+  if (bytes == partBytes(LOADS)) {
+    u32x4 v[LOADS];
 #pragma unroll
-    for (int u = 0; u < kPartLoads; u++) v[u] = load16<1>(from + (u * 64 + lane) * 16);
+    for (int u = 0; u < LOADS; u++) v[u] = load16<1, NT>(from + (u * 64 + lane) * 16);
 #pragma unroll
-    for (int u = 0; u < kPartLoads; u++) store16<1, true>(to + (u * 64 + lane) * 16, v[u]);
+    for (int u = 0; u < LOADS; u++) store16<1, true>(to + (u * 64 + lane) * 16, v[u]);
     return;
   }
   const uint32_t packs = bytes / 16;
@@ -299,14 +303,19 @@ __device__ __forceinline__ MoveItem itemOf(const PoolSet& p, uint64_t item, uint
   m.part = (uint32_t)(in - (uint64_t)m.move * p.parts);
   return m;
 }
+template <int LOADS, bool NT>
 __device__ __forceinline__ void moveItem(const PoolSet& p, int32_t src, int32_t dst, const MoveItem& m, int lane) {
-  const size_t at = (size_t)m.part * kPartBytes;
+  const size_t at = (size_t)m.part * partBytes(LOADS);
   // (the last part's size comes from the host: the minimum of two 64-bit sizes that are the same in every lane is
   // compiled into a vector compare whose result the scalar select that follows does not read)
-  const uint32_t bytes = m.part + 1 == p.parts ? p.lastBytes : kPartBytes;
-  movePart(p.from[m.pool] + (size_t)src * p.pageBytes + at, p.to[m.pool] + (size_t)dst * p.pageBytes + at, bytes, (uint32_t)lane);
+  const uint32_t bytes = m.part + 1 == p.parts ? p.lastBytes : partBytes(LOADS);
+  movePart<LOADS, NT>(p.from[m.pool] + (size_t)src * p.pageBytes + at, p.to[m.pool] + (size_t)dst * p.pageBytes + at, bytes,
+                      (uint32_t)lane);
 }
 
+// 300 pages of 32 KiB in 64 pools, 1.26 GB of traffic: 208 us = 6.0 TB/s, as much as the library's dense copy reaches
+// (6.1). What that took: workgroups that move 4 KiB and end (16 KiB: 228 us; a fixed number of workgroups that walk the
+// pages: 255), pool by pool (pair by pair 14 us more), stores that do not stay in the caches (18 us).
 __global__ __launch_bounds__(kMoveThreads) void copyKernel(PoolSet p, const int32_t* srcPages, const int32_t* dstPages,
                                                            int32_t n, int32_t srcTotal, int32_t dstTotal) {
   const int lane = (int)(threadIdx.x & 63);
@@ -316,10 +325,12 @@ __global__ __launch_bounds__(kMoveThreads) void copyKernel(PoolSet p, const int3
     const MoveItem m = itemOf(p, item, (uint32_t)n);
     const int32_t src = uniform(srcPages[m.move]), dst = uniform(dstPages[m.move]);
     if (src < 0 || src >= srcTotal || dst < 0 || dst >= dstTotal) continue;
-    moveItem(p, src, dst, m, lane);
+    moveItem<kCopyLoads, false>(p, src, dst, m, lane);
   }
 }
 
+// 512 forks of 8 pools' 16 KiB pages: 16 children read the same page, so loads stay in the caches (25 us for the call; 39
+// if they do not). Two loads a lane: 25 us, four 27, one 33 (every wave looks its request up).
 // Fork. The first q.n workgroups (of the first launch, if the pools take several) write the tables, one per request:
 // the child's whole pages are the parent's, a last page that is not full is the child's own. The others copy the
 // contents of those. Neither reads what the other writes: children were empty, and parents stay as they are.
@@ -359,7 +370,7 @@ __global__ __launch_bounds__(kMoveThreads) void forkKernel(Books b, PageScratch 
     if (first < 0 || before % b.pageTokens == 0 || first >= uniform(s.counts[0])) continue;
     const int32_t src = uniform(b.tables[(size_t)uniform(q.a[m.move]) * b.perSeq + before / b.pageTokens]);
     if (src < 0 || src >= b.pages) continue;
-    moveItem(p, src, uniform(s.found[first]), m, lane);
+    moveItem<kForkLoads, false>(p, src, uniform(s.found[first]), m, lane);
   }
 }
 
@@ -492,6 +503,9 @@ __global__ __launch_bounds__(kScanThreads) void listMovesKernel(Books b, PageScr
   }
 }
 
+// 1000 moves of 16 pools' 16 KiB pages, 96 us for the call: the pages are read and written at 5.6 TB/s. How many move is
+// known on the GPU only, so a grid of at most kMaxCompactGrid walks them: 96 us; 2048 workgroups 105. Four loads a lane
+// that do not stay in the caches: 98 us in that sweep, two 103, one 105; loads that stay 104.
 // Compact, the moves: the first bookBlocks workgroups (of the first launch) let table entries and counts follow, the
 // others move the contents.
 __global__ __launch_bounds__(kMoveThreads) void compactKernel(Books b, PageScratch s, PoolSet p, uint32_t bookBlocks) {
@@ -522,7 +536,7 @@ __global__ __launch_bounds__(kMoveThreads) void compactKernel(Books b, PageScrat
   for (uint64_t item = (uint64_t)(blockIdx.x - bookBlocks) * kMoveWaves + waveInBlock(); item < items;
        item += (uint64_t)(gridDim.x - bookBlocks) * kMoveWaves) {
     const MoveItem m = itemOf(p, item, (uint32_t)moves);
-    moveItem(p, uniform(s.movers[m.move]), uniform(s.found[m.move]), m, lane);
+    moveItem<kCompactLoads, true>(p, uniform(s.movers[m.move]), uniform(s.found[m.move]), m, lane);
   }
 }
 
@@ -594,7 +608,7 @@ static PageScratch scratchOf(const dfcclPageCache* c) {
   s.counts = (int32_t*)(ws + p.counts);
   return s;
 }
-static PoolSet poolSet(const dfcclPageCache* to, const dfcclPageCache* from, int first) {
+static PoolSet poolSet(const dfcclPageCache* to, const dfcclPageCache* from, int first, int loads) {
   PoolSet p{};
   p.npools = std::min(kMaxPools, to->npools - first);
   for (int i = 0; i < p.npools; i++) {
@@ -602,11 +616,12 @@ static PoolSet poolSet(const dfcclPageCache* to, const dfcclPageCache* from, int
     p.from[i] = (const char*)from->pools[first + i];
   }
   p.pageBytes = to->pageBytes;
-  p.parts = (uint32_t)((to->pageBytes + kPartBytes - 1) / kPartBytes);
-  p.lastBytes = (uint32_t)(to->pageBytes - (size_t)(p.parts - 1) * kPartBytes);
+  p.parts = (uint32_t)((to->pageBytes + partBytes(loads) - 1) / partBytes(loads));
+  p.lastBytes = (uint32_t)(to->pageBytes - (size_t)(p.parts - 1) * partBytes(loads));
   return p;
 }
 constexpr uint64_t kMaxMoveGrid = 1u << 22;
+constexpr unsigned kMaxCompactGrid = 1u << 16;
 static unsigned moveGrid(uint64_t items) {
   return (unsigned)std::max<uint64_t>(1, std::min<uint64_t>((items + kMoveWaves - 1) / kMoveWaves, kMaxMoveGrid));
 }
@@ -626,7 +641,7 @@ static bool launchAssign(const Books& b, const PageScratch& s, const Requests& q
 }
 static ncclResult_t launched() { return hipGetLastError() == hipSuccess ? ncclSuccess : ncclUnhandledCudaError; }
 // a page's parts over a launch's pools are counted in 32 bits
-static bool soundPage(const dfcclPageCache* c) { return c->pageBytes <= ((size_t)1 << 36); }  // (2^24 parts, 64 pools)
+static bool soundPage(const dfcclPageCache* c) { return c->pageBytes <= ((size_t)1 << 36); }  // (2^26 parts, 64 pools)
 
 }  // namespace dfccl
 
@@ -647,7 +662,7 @@ DFCCL_API ncclResult_t dfcclPagesCopy(const dfcclPageCache* to, const dfcclPageC
   if (n == 0) return ncclSuccess;
   if (srcPages == nullptr || dstPages == nullptr) return ncclInvalidArgument;
   for (int first = 0; first < to->npools; first += kMaxPools) {
-    const PoolSet p = poolSet(to, from, first);
+    const PoolSet p = poolSet(to, from, first, kCopyLoads);
     DFCCL_LAUNCH_BLOCKS(copyKernel, moveGrid((uint64_t)n * p.npools * p.parts), kMoveThreads, (hipStream_t)stream, p, srcPages,
                         dstPages, n, from->pages, to->pages);
   }
@@ -677,7 +692,7 @@ DFCCL_API ncclResult_t dfcclPagesFork(const dfcclPageCache* c, const int32_t* pa
   const Requests q{parents, children, n};
   (void)launchAssign<kForFork>(b, s, q, st);
   for (int first = 0; n > 0 && first < c->npools; first += kMaxPools) {
-    const PoolSet p = poolSet(c, c, first);
+    const PoolSet p = poolSet(c, c, first, kForkLoads);
     const unsigned tableBlocks = first == 0 ? (unsigned)n : 0u;
     DFCCL_LAUNCH_BLOCKS(forkKernel, tableBlocks + moveGrid((uint64_t)n * p.npools * p.parts), kMoveThreads, st, b, s, q, p,
                         tableBlocks);
@@ -705,11 +720,11 @@ DFCCL_API ncclResult_t dfcclPagesCompact(const dfcclPageCache* c, void* stream) 
     DFCCL_LAUNCH_BLOCKS(listMovesKernel, (unsigned)tiles, kScanThreads, st, b, s, tiles);
   }
   for (int first = 0; first < c->npools; first += kMaxPools) {
-    const PoolSet p = poolSet(c, c, first);
+    const PoolSet p = poolSet(c, c, first, kCompactLoads);
     // how many pages move is known on the GPU only: at most half of them
     const uint64_t most = (uint64_t)(c->pages / 2) * p.npools * p.parts;
     const unsigned bookBlocks = first == 0 ? (unsigned)std::min(c->sequences, 2048) : 0u;
-    DFCCL_LAUNCH_BLOCKS(compactKernel, bookBlocks + std::min(moveGrid(most), 2048u), kMoveThreads, st, b, s, p, bookBlocks);
+    DFCCL_LAUNCH_BLOCKS(compactKernel, bookBlocks + std::min(moveGrid(most), kMaxCompactGrid), kMoveThreads, st, b, s, p, bookBlocks);
   }
   return launched();
 }

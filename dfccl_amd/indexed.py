@@ -34,24 +34,37 @@ def _call(device, fn, what, *args):
         api.check(code, what)
 
 
-def _rows_ptr(t, what):
-    """Address and row stride (in elements) of a 2-d tensor whose rows are contiguous."""
+def _ptr(t):
+    return t.data_ptr() if t.is_cuda else api._dev_ptr(t)
+
+
+def _row_stride(t, what):
+    """Row stride (in elements) of a 2-d tensor whose rows are contiguous and do not overlap."""
     if t.dim() != 2:
         raise ValueError(f"{what} must have two dimensions")
+    rows, width = t.shape
+    stride, inner = t.stride()
+    if rows > 1 and stride < width or width > 1 and inner != 1:
+        if not t.is_contiguous():  # (strides of a tensor without elements mean nothing)
+            raise ValueError(f"{what}: the elements of a row must be contiguous, and rows must not overlap")
+    return stride if rows > 1 and stride > width else width
+
+
+def _rows_ptr(t, what):
+    """Address and row stride of a table, an output or a gradient."""
     if t.dtype not in _FLOATS:
         raise TypeError(f"{what}: dtype {t.dtype} is not one of float32, float16, bfloat16")
-    if t.is_contiguous():
-        return t.data_ptr() if t.is_cuda else api._dev_ptr(t), t.shape[1]
-    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-        raise ValueError(f"{what}: the elements of a row must be contiguous, and rows must not overlap")
-    return api._dev_ptr(t[0]), t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return _ptr(t), _row_stride(t, what)
 
 
 def _ids_ptr(ids, device):
     if ids.dtype is not torch.int64 and ids.dtype is not torch.int32:
         raise TypeError(f"ids: dtype {ids.dtype} is not int32 or int64")
-    _on(device, ids)
-    return api._dev_ptr(ids)
+    if ids.device != device:
+        _on(device, ids)
+    if not ids.is_contiguous():
+        raise ValueError("ids must be contiguous")
+    return _ptr(ids)
 
 
 def _on(device, *tensors):
@@ -98,19 +111,21 @@ def embedding_grad(grads, ids, table_grad, scale=1.0, first_row=0, padding_id=No
     table_ptr, table_stride = _rows_ptr(table_grad, "table_grad")
     rows, width = table_grad.shape
     device, dtype, id_type = table_grad.device, grads[0].dtype, ids[0].dtype
+    if dtype not in _FLOATS:
+        raise TypeError(f"grads: dtype {dtype} is not one of float32, float16, bfloat16")
     grad_ptrs, id_ptrs, sizes = (ctypes.c_void_p * n)(), (ctypes.c_void_p * n)(), (ctypes.c_size_t * n)()
     grad_stride = None
     for r in range(n):
         g, i = grads[r], ids[r]
-        grad_ptrs[r], stride = _rows_ptr(g, "grads")
-        id_ptrs[r] = _ids_ptr(i, device)
-        if g.dtype != dtype or i.dtype != id_type:
+        if g.dtype is not dtype or i.dtype is not id_type:
             raise ValueError("the sources must agree in dtype")
         tokens = i.numel()
-        if tuple(g.shape) != (tokens, width):
+        stride = _row_stride(g, "grads")
+        if g.shape[0] != tokens or g.shape[1] != width:
             raise ValueError(f"grads[{r}] has shape {tuple(g.shape)}, not {(tokens, width)}")
-        _on(device, g)
-        sizes[r] = tokens
+        if g.device != device:
+            _on(device, g)
+        grad_ptrs[r], id_ptrs[r], sizes[r] = _ptr(g), _ids_ptr(i, device), tokens
         if tokens > 1:
             if grad_stride is not None and grad_stride != stride:
                 raise ValueError("the sources must agree in their row stride")
@@ -137,32 +152,33 @@ class PageCache:
     requests refused by the last extend or fork; report[1], report[2]: pages moved, pages live at the last compact."""
 
     def __init__(self, pools, page_tokens, refcounts, tables, lengths):
-        pages, size = pools[0].shape[0], pools[0].numel() * pools[0].element_size()
-        device = refcounts.device
-        for p in pools:
-            if p.shape[0] != pages or p.numel() * p.element_size() != size:
+        pages, size, device = pools[0].shape[0], pools[0].nbytes, refcounts.device
+        pointers = (ctypes.c_void_p * len(pools))()
+        for k, p in enumerate(pools):
+            if p.nbytes != size or p.shape[0] != pages:
                 raise ValueError("the pools must agree in pages and bytes per page")
+            if p.device != device:
+                _on(device, p)
+            pointers[k] = p.data_ptr() if p.is_cuda and p.is_contiguous() else api._dev_ptr(p)
         for t in (refcounts, tables, lengths):
             if t.dtype != torch.int32:
                 raise TypeError("the bookkeeping is held in int32 tensors")
         if refcounts.shape != (pages,) or tables.dim() != 2 or lengths.shape != (tables.shape[0],):
             raise ValueError("refcounts is [pages], tables [sequences, pages per sequence], lengths [sequences]")
-        _on(device, tables, lengths, *pools)
+        _on(device, tables, lengths)
         lib = _lib.load()
         need = ctypes.c_size_t()
         api.check(lib.dfcclPageCacheWorkspace(pages, tables.shape[0], ctypes.byref(need)), "dfcclPageCacheWorkspace")
         self.pools, self.page_tokens = pools, page_tokens
         self.refcounts, self.tables, self.lengths = refcounts, tables, lengths
         self.report = torch.zeros(3, dtype=torch.int32, device=device)
-        self._device = device
+        self._device, self._lib, self._pointers = device, lib, pointers
         self._workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
-        self._pointers = (ctypes.c_void_p * len(pools))(*[api._dev_ptr(p).value for p in pools])
         self._struct = _lib.PageCacheStruct(
-            ctypes.sizeof(_lib.PageCacheStruct), self._pointers, size // max(1, pages), len(pools), pages, page_tokens,
+            ctypes.sizeof(_lib.PageCacheStruct), pointers, size // max(1, pages), len(pools), pages, page_tokens,
             tables.shape[0], tables.shape[1], api._dev_ptr(refcounts), api._dev_ptr(tables), api._dev_ptr(lengths),
             api._dev_ptr(self.report), api._dev_ptr(self._workspace), need.value)
         self._ref = ctypes.byref(self._struct)
-        self._lib = lib
 
     @classmethod
     def empty(cls, pools, page_tokens, sequences, pages_per_sequence):

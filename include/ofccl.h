@@ -197,7 +197,8 @@ ncclResult_t dfcclReduceCopy(const void* const* srcs, int nsrcs, void* dst, size
  * firstRow (>= 0); an id outside the piece names no row.  Tables, outputs and
  * gradients are ncclFloat32, ncclFloat16 or ncclBfloat16, each of its own type
  * and aligned to it; ids are ncclInt32 or ncclInt64.  Strides are in elements,
- * from row to row, at least `width`.  Up to 2^31-1 tokens, rows and columns.
+ * from row to row, at least `width`.  Fewer than 2^31 tokens, rows and columns
+ * each.  What is written must not overlap what is read.
  * Asynchronous on `stream`, allocate nothing, may be captured into a graph. */
 
 /* out[t,:] = scale * table[id_t - firstRow,:], computed in fp32 and rounded

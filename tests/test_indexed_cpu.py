@@ -107,6 +107,17 @@ def test_pages_refuse():
     assert L.dfcclPagesCopy(bare, ctypes.byref(cache(npools=1)), PTR, PTR, 1, None) == INVALID
 
 
+@pytest.mark.skipif(not os.path.exists("/opt/rocm/bin/hipcc"), reason="needs hipcc")
+@pytest.mark.parametrize("source", ["embedding", "pages"])
+def test_kernels_use_no_scratch_and_spill_no_vector_registers(source):
+    from test_kernel_resources_cpu import resources
+    kernels = resources(source)
+    assert len(kernels) >= 10
+    for name, k in kernels.items():
+        assert int(k["ScratchSize [bytes/lane]"]) == 0 and k["Dynamic Stack"] == "False", name
+        assert int(k["VGPRs Spill"]) == 0, name
+
+
 CLANG = "/opt/rocm/lib/llvm/bin/clang++"
 
 

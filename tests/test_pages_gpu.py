@@ -166,8 +166,9 @@ def test_compact_and_extend_over_several_rounds_of_the_scan(pages):
     both.compact()
 
 
-# page sizes around a wave's 4096 bytes and the 16 bytes of a load; pools around the 64 of a launch
-@pytest.mark.parametrize("page_bytes,npools", [(1, 1), (15, 3), (16, 2), (17, 2), (4095, 1), (4096, 2), (4097, 2), (8195, 1),
+# page sizes around a wave's 1024, 2048 and 4096 bytes and the 16 bytes of a load; pools around the 64 of a launch
+@pytest.mark.parametrize("page_bytes,npools", [(1, 1), (15, 3), (16, 2), (17, 2), (1023, 1), (1024, 1), (1025, 1), (2047, 1),
+                                               (2048, 1), (2049, 1), (4095, 1), (4096, 2), (4097, 2), (8195, 1),
                                                (8, 64), (6, 65), (32, 131)])
 def test_contents_of_odd_pages_and_many_pools(page_bytes, npools):
     import dfccl_amd
