@@ -205,21 +205,39 @@ __device__ __forceinline__ void clearShare(const Clear& c) {
   }
 }
 
-__device__ __forceinline__ void keyOfToken(const GradArgs& a, uint32_t pos, uint32_t& key, uint32_t& pay) {
-  int r = 0;
-  const char* ids = a.ids[0];
-  uint32_t first = 0;
+// The keys and payloads of S positions before sorting (of the last one, for positions behind it). The ids are loaded
+// without conditions, all of them at once: under one, each load would be waited for by itself.
+template <int S>
+__device__ __forceinline__ void keysOfTokens(const GradArgs& a, const uint32_t (&pos)[S], uint32_t (&key)[S], uint32_t (&pay)[S]) {
+  const char* at[S];
 #pragma unroll
-  for (int i = 1; i < kMaxSrcs; i++)
-    if (i < a.nsrcs && pos >= a.firstPos[i]) {
-      r = i;
-      ids = a.ids[i];
-      first = a.firstPos[i];
+  for (int k = 0; k < S; k++) {
+    const uint32_t p = pos[k] < a.n ? pos[k] : a.n - 1;
+    uint32_t r = 0, first = 0;
+    const char* ids = a.ids[0];
+#pragma unroll
+    for (int i = 1; i < kMaxSrcs; i++) {
+      const bool behind = i < a.nsrcs && p >= a.firstPos[i];
+      r = behind ? (uint32_t)i : r;
+      ids = behind ? a.ids[i] : ids;
+      first = behind ? a.firstPos[i] : first;
     }
-  const uint32_t t = pos - first;
-  const int64_t id = loadId(ids, a.idBytes, t), row = rowOf(id, a.firstRow, a.rows);
-  key = row >= 0 && id != a.paddingId ? (uint32_t)row : a.rows;
-  pay = ((uint32_t)r << kSrcShift) | t;
+    pay[k] = (r << kSrcShift) | (p - first);
+    at[k] = ids + (size_t)(p - first) * a.idBytes;
+  }
+  int64_t id[S];
+  if (a.idBytes == 8) {
+#pragma unroll
+    for (int k = 0; k < S; k++) id[k] = *(const DFCCL_GLOBAL int64_t*)at[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < S; k++) id[k] = *(const DFCCL_GLOBAL int32_t*)at[k];
+  }
+#pragma unroll
+  for (int k = 0; k < S; k++) {
+    const int64_t row = rowOf(id[k], a.firstRow, a.rows);
+    key[k] = row >= 0 && id[k] != a.paddingId ? (uint32_t)row : a.rows;
+  }
 }
 __device__ __forceinline__ uint32_t payOf(const GradArgs& a, uint32_t pos) {
   uint32_t r = 0, first = 0;
@@ -237,19 +255,20 @@ __device__ __forceinline__ uint32_t payOf(const GradArgs& a, uint32_t pos) {
 __device__ __forceinline__ uint64_t sameDigit(uint32_t digit, int bits, bool valid) {
   uint64_t same = __ballot(valid);
   for (int b = 0; b < bits; b++) {
-    const bool one = (digit >> b) & 1u;
-    const uint64_t ones = __ballot(one);
-    same &= one ? ones : ~ones;
+    const uint64_t ones = __ballot((digit >> b) & 1u);
+    const uint64_t mine = (uint64_t)(int64_t)((int32_t)(digit << (31 - b)) >> 31);  // the lane's bit in all 64
+    same &= ~(ones ^ mine);
   }
   return same;
 }
 // The rank of a strip's keys among the wave's keys of the same digit so far, whose counts are kept in LDS.
-__device__ __forceinline__ uint32_t rankInWave(uint32_t* count, uint32_t digit, int bits, bool valid, int lane) {
+template <typename C>
+__device__ __forceinline__ uint32_t rankInWave(C* count, uint32_t digit, int bits, bool valid, int lane) {
   const uint64_t same = sameDigit(digit, bits, valid);
   const uint64_t before = same & ((1ull << lane) - 1);
   const uint32_t old = count[digit];
   DFCCL_WAVE_LDS_SYNC();  // (every lane has read the count before the first of its digit raises it)
-  if (valid && before == 0) count[digit] = old + (uint32_t)__builtin_popcountll(same);
+  if (valid && before == 0) count[digit] = (C)(old + (uint32_t)__builtin_popcountll(same));
   DFCCL_WAVE_LDS_SYNC();
   return old + (uint32_t)__builtin_popcountll(before);
 }
@@ -262,34 +281,34 @@ __device__ __forceinline__ uint32_t waveScan(uint32_t v, int lane) {  // inclusi
   return v;
 }
 
-// ---- up to 16384 tokens: sorted by one workgroup in LDS, one launch instead of two per digit. Bound by the latency of
-// its steps (per digit six barriers and a ballot per bit and 64 keys): 12 us for 3600 tokens and 14 bits, where counts
-// and scatters took 23 in four launches; 52 us for 16384 tokens and 18 bits, where those took 38, but there one launch
-// lets the table's clearing (167 us for 1 GiB) run beside it without a break: 253 instead of 282 us for the whole call.
+// ---- a few thousand tokens: sorted by one workgroup in LDS, one launch instead of two per digit. Bound by the latency
+// of its steps and by the instructions of one compute unit (a ballot per bit and 64 keys): 12 us for 3600 tokens and 14
+// bits, where counts and scatters take 21; 40 us for 13000 tokens, where those take 22.
 constexpr int kSmallThreads = 1024;
 constexpr int kSmallWaves = kSmallThreads / 64;
-constexpr int kFewStrips = 4, kManyStrips = 16;
+constexpr int kSmallStrips = 4;
 // (a host build sets lower limits, to reach with few tokens what lies beyond them)
 #ifndef DFCCL_SORT_SMALL_MAX
-#define DFCCL_SORT_SMALL_MAX (kSmallThreads * kManyStrips)
+#define DFCCL_SORT_SMALL_MAX (kSmallThreads * kSmallStrips)
 #endif
 #ifndef DFCCL_SUPER_MIN
 #define DFCCL_SUPER_MIN 8192
 #endif
 constexpr uint32_t kSmallMax = DFCCL_SORT_SMALL_MAX, kSuperMin = DFCCL_SUPER_MIN;
-static_assert(kSmallMax <= kSmallThreads * kManyStrips, "one workgroup sorts no more");
-constexpr int kSmallDigitBits = 8;
+static_assert(kSmallMax <= kSmallThreads * kSmallStrips, "one workgroup sorts no more");
+constexpr int kSmallDigitBits = 10;
 constexpr int kSmallBins = 1 << kSmallDigitBits;
+static_assert(kSmallBins == kSmallThreads, "a thread per bin");
 
-template <int S>
 __global__ __launch_bounds__(kSmallThreads) void sortSmallKernel(GradArgs a, int keyBits, Clear c) {
+  constexpr int S = kSmallStrips;
   struct Shared {
     uint32_t key[kSmallThreads * S];
     uint16_t pos[kSmallThreads * S];  // before sorting
-    uint32_t count[kSmallWaves][kSmallBins];
-    uint32_t waveTotal[kSmallBins / 64];
+    uint16_t count[kSmallWaves][kSmallBins];
+    uint32_t waveTotal[kSmallWaves];
   };
-  static_assert(kSmallThreads * kManyStrips <= 65536, "positions are held in 16 bits");
+  static_assert(kSmallThreads * S < 65536, "positions and counts are held in 16 bits");
   DFCCL_WG_SHARED(Shared, sh);
   if (blockIdx.x >= c.firstBlock) {
     clearShare<kSmallWaves>(c);
@@ -299,17 +318,17 @@ __global__ __launch_bounds__(kSmallThreads) void sortSmallKernel(GradArgs a, int
   const uint32_t start = (uint32_t)wave * (64 * S);
   uint32_t key[S], pos[S], rank[S];
 #pragma unroll
-  for (int k = 0; k < S; k++) {
-    uint32_t pay;
-    pos[k] = start + k * 64 + lane;
-    key[k] = 0;
-    if (pos[k] < a.n) keyOfToken(a, pos[k], key[k], pay);
-  }
+  for (int k = 0; k < S; k++) pos[k] = start + k * 64 + lane;
+  if (start < a.n) keysOfTokens<S>(a, pos, key, rank);  // (payloads are made from positions at the end)
   const int passes = (keyBits + kSmallDigitBits - 1) / kSmallDigitBits, bits = (keyBits + passes - 1) / passes;
   for (int pass = 0; pass < passes; pass++) {
     const int shift = pass * bits;
     const uint32_t mask = (1u << bits) - 1;
-    for (int i = tid; i < kSmallWaves * kSmallBins; i += kSmallThreads) sh.count[i / kSmallBins][i % kSmallBins] = 0;
+    const int bins = 1 << bits;
+    if (tid < bins) {
+#pragma unroll
+      for (int w = 0; w < kSmallWaves; w++) sh.count[w][tid] = 0;
+    }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < S; k++)
@@ -317,21 +336,21 @@ __global__ __launch_bounds__(kSmallThreads) void sortSmallKernel(GradArgs a, int
         rank[k] = rankInWave(sh.count[wave], (key[k] >> shift) & mask, bits, start + k * 64 + lane < a.n, lane);
     __syncthreads();
     // a digit's keys begin behind all keys of smaller digits, a wave's behind the same digit's of the waves before
-    uint32_t mine = 0, sum = 0;
-    if (tid < kSmallBins) {
+    uint32_t mine = 0;
+    if (tid < bins) {
 #pragma unroll
       for (int w = 0; w < kSmallWaves; w++) mine += sh.count[w][tid];
-      sum = waveScan(mine, lane);
-      if (lane == 63) sh.waveTotal[wave] = sum;
     }
+    const uint32_t sum = waveScan(mine, lane);
+    if (lane == 63) sh.waveTotal[wave] = sum;
     __syncthreads();
-    if (tid < kSmallBins) {
-      uint32_t at = sum - mine;
-      for (int w = 0; w < wave; w++) at += sh.waveTotal[w];
+    uint32_t at = sum - mine;
+    for (int w = 0; w < wave; w++) at += sh.waveTotal[w];
+    if (tid < bins) {
 #pragma unroll
       for (int w = 0; w < kSmallWaves; w++) {
         const uint32_t n = sh.count[w][tid];
-        sh.count[w][tid] = at;
+        sh.count[w][tid] = (uint16_t)at;
         at += n;
       }
     }
@@ -363,12 +382,31 @@ __global__ __launch_bounds__(kSmallThreads) void sortSmallKernel(GradArgs a, int
   }
 }
 
-// ---- more tokens: tiles, a count and a scatter per digit (5 and 15 us at 16384 tokens)
+// ---- more tokens: tiles, a count and a scatter per digit (4 and 7 us at 13000 tokens, of which the launches are half)
 constexpr int kSortThreads = 256;
 constexpr int kSortWaves = kSortThreads / 64;
-// strips of a tile: few enough that some ten thousand tokens spread over several workgroups, many enough that
-// the sum over the tiles' histograms, which every tile makes for itself, stays short
-constexpr int kShortStrips = 4, kLongStrips = 16;
+// 64-key strips of a wave of a tile: few enough that the tokens spread over several workgroups, many enough that there
+// are not more than a few dozen histograms, which every tile adds up for itself (2 instead of 4 strips: 40 instead of
+// 42 us for a call on 13000 tokens)
+static int stripsOf(uint64_t n) { return n <= 16u * 1024 ? 2 : n <= 64u * 1024 ? 4 : 16; }
+
+// The keys and payloads of a tile's strips before the first pass, a few strips at a time.
+template <int S>
+__device__ __forceinline__ void tileKeys(const GradArgs& a, const uint32_t (&pos)[S], uint32_t (&key)[S], uint32_t (&pay)[S]) {
+  constexpr int N = S < 4 ? S : 4;
+#pragma unroll
+  for (int g = 0; g < S; g += N) {
+    uint32_t p[N], k[N], y[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) p[i] = pos[g + i];
+    keysOfTokens<N>(a, p, k, y);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      key[g + i] = k[i];
+      pay[g + i] = y[i];
+    }
+  }
+}
 
 template <int S, bool FIRST>
 __global__ __launch_bounds__(kSortThreads) void sortCountKernel(GradArgs a, SortPass p, Clear c) {
@@ -383,16 +421,19 @@ __global__ __launch_bounds__(kSortThreads) void sortCountKernel(GradArgs a, Sort
   const int tid = (int)threadIdx.x, tile = (int)blockIdx.x, bins = 1 << p.bits;
   for (int i = tid; i < bins; i += kSortThreads) sh.count[i] = 0;
   __syncthreads();
+  uint32_t pos[S], key[S], pay[S];  // (positions of a launch fit 32 bits: there are fewer than 2^31 tokens)
 #pragma unroll
-  for (int k = 0; k < S; k++) {
-    const uint64_t pos = (uint64_t)tile * (kSortThreads * S) + k * kSortThreads + tid;
-    if (pos < a.n) {
-      uint32_t key, pay;
-      if constexpr (FIRST) keyOfToken(a, (uint32_t)pos, key, pay);
-      else key = a.keys[p.from][pos];
-      __hip_atomic_fetch_add(&sh.count[(key >> p.shift) & (bins - 1)], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-    }
+  for (int k = 0; k < S; k++) pos[k] = (uint32_t)tile * (kSortThreads * S) + k * kSortThreads + tid;
+  if constexpr (FIRST) {
+    tileKeys<S>(a, pos, key, pay);
+  } else {
+#pragma unroll
+    for (int k = 0; k < S; k++) key[k] = a.keys[p.from][pos[k] < a.n ? pos[k] : a.n - 1];
   }
+#pragma unroll
+  for (int k = 0; k < S; k++)
+    if (pos[k] < a.n)
+      __hip_atomic_fetch_add(&sh.count[(key[k] >> p.shift) & (bins - 1)], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
   __syncthreads();
   for (int i = tid; i < bins; i += kSortThreads) a.hist[(size_t)tile * bins + i] = sh.count[i];
 }
@@ -413,18 +454,17 @@ __global__ __launch_bounds__(kSortThreads) void sortScatterKernel(GradArgs a, So
     return;
   }
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = waveInBlock(), tile = (int)blockIdx.x, bins = 1 << p.bits;
-  uint32_t key[S], pay[S], rank[S];
-  const uint64_t start = (uint64_t)tile * (kSortThreads * S) + (uint64_t)wave * (64 * S) + lane;
+  uint32_t pos[S], key[S], pay[S], rank[S];
 #pragma unroll
-  for (int k = 0; k < S; k++) {
-    const uint64_t pos = start + k * 64;
-    key[k] = pay[k] = 0;
-    if (pos < a.n) {
-      if constexpr (FIRST) keyOfToken(a, (uint32_t)pos, key[k], pay[k]);
-      else {
-        key[k] = a.keys[p.from][pos];
-        pay[k] = a.pays[p.from][pos];
-      }
+  for (int k = 0; k < S; k++) pos[k] = (uint32_t)tile * (kSortThreads * S) + (uint32_t)wave * (64 * S) + k * 64 + lane;
+  if constexpr (FIRST) {
+    tileKeys<S>(a, pos, key, pay);
+  } else {
+#pragma unroll
+    for (int k = 0; k < S; k++) {
+      const uint32_t at = pos[k] < a.n ? pos[k] : a.n - 1;
+      key[k] = a.keys[p.from][at];
+      pay[k] = a.pays[p.from][at];
     }
   }
   for (int i = tid; i < kMaxBins; i += kSortThreads) {
@@ -445,7 +485,7 @@ __global__ __launch_bounds__(kSortThreads) void sortScatterKernel(GradArgs a, So
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < S; k++)
-    rank[k] = rankInWave(sh.count[wave], (key[k] >> p.shift) & (uint32_t)(bins - 1), p.bits, start + k * 64 < a.n, lane);
+    rank[k] = rankInWave(sh.count[wave], (key[k] >> p.shift) & (uint32_t)(bins - 1), p.bits, pos[k] < a.n, lane);
   constexpr int per = kMaxBins / kSortThreads;
   uint32_t mine = 0;
 #pragma unroll
@@ -470,7 +510,7 @@ __global__ __launch_bounds__(kSortThreads) void sortScatterKernel(GradArgs a, So
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < S; k++)
-    if (start + k * 64 < a.n) {
+    if (pos[k] < a.n) {
       const uint32_t to = sh.count[wave][(key[k] >> p.shift) & (uint32_t)(bins - 1)] + rank[k];
       a.keys[p.from ^ 1][to] = key[k];
       a.pays[p.from ^ 1][to] = pay[k];
@@ -783,9 +823,10 @@ template <int S, bool FIRST>
 static SortKernel pickSortS(bool scatter) {
   return scatter ? sortScatterKernel<S, FIRST> : sortCountKernel<S, FIRST>;
 }
-static SortKernel pickSort(bool scatter, bool longTiles, bool first) {
-  if (longTiles) return first ? pickSortS<kLongStrips, true>(scatter) : pickSortS<kLongStrips, false>(scatter);
-  return first ? pickSortS<kShortStrips, true>(scatter) : pickSortS<kShortStrips, false>(scatter);
+static SortKernel pickSort(bool scatter, int strips, bool first) {
+  if (strips == 2) return first ? pickSortS<2, true>(scatter) : pickSortS<2, false>(scatter);
+  if (strips == 4) return first ? pickSortS<4, true>(scatter) : pickSortS<4, false>(scatter);
+  return first ? pickSortS<16, true>(scatter) : pickSortS<16, false>(scatter);
 }
 typedef void (*RowsKernel)(GradArgs, int);
 template <bool NARROW>
@@ -812,8 +853,8 @@ static RowsKernel pickRows(int gt, int tt, bool accumulate, bool narrow) {
 
 // Plan of a gradient call from its sizes: how it is sorted and where the workspace's parts begin.
 struct GradPlan {
-  bool small, longTiles, chunked, supered;
-  int keyBits, passes, digitBits, tiles;
+  bool small, chunked, supered;
+  int keyBits, passes, digitBits, strips, tiles;
   size_t keys[2], pays[2], hist, chunkSums, superSums, bytes;
 };
 static GradPlan planGrad(uint64_t n, size_t rows, size_t width) {
@@ -823,8 +864,8 @@ static GradPlan planGrad(uint64_t n, size_t rows, size_t width) {
   p.small = n <= kSmallMax;
   p.passes = (p.keyBits + kMaxDigitBits - 1) / kMaxDigitBits;
   p.digitBits = (p.keyBits + p.passes - 1) / p.passes;
-  p.longTiles = n > 64u * 1024;
-  const uint64_t tile = (uint64_t)kSortThreads * (p.longTiles ? kLongStrips : kShortStrips);
+  p.strips = stripsOf(n);
+  const uint64_t tile = (uint64_t)kSortThreads * p.strips;
   p.tiles = (int)std::max<uint64_t>(1, (n + tile - 1) / tile);
   // Runs of fewer than 64 tokens need no chunks. Chunks of chunks pay for their launch once a run may have several
   // hundred chunks.
@@ -990,14 +1031,13 @@ DFCCL_API ncclResult_t dfcclEmbeddingGrad(const void* const* grads, const void* 
   int from = 0;
   if (p.small) {
     const unsigned grid = share(1);
-    DFCCL_LAUNCH_BLOCKS((n <= kSmallThreads * kFewStrips ? sortSmallKernel<kFewStrips> : sortSmallKernel<kManyStrips>), grid,
-                        kSmallThreads, st, a, p.keyBits, clear);
+    DFCCL_LAUNCH_BLOCKS(sortSmallKernel, grid, kSmallThreads, st, a, p.keyBits, clear);
   }
   for (int pass = 0; !p.small && pass < p.passes; pass++, from ^= 1) {
     const SortPass s{from, pass * p.digitBits, p.digitBits, p.tiles};
     for (int scatter = 0; scatter < 2; scatter++) {
       const unsigned grid = share((unsigned)p.tiles);
-      DFCCL_LAUNCH_BLOCKS(pickSort(scatter != 0, p.longTiles, pass == 0), grid, kSortThreads, st, a, s, clear);
+      DFCCL_LAUNCH_BLOCKS(pickSort(scatter != 0, p.strips, pass == 0), grid, kSortThreads, st, a, s, clear);
     }
   }
   if (p.chunked)

@@ -269,9 +269,9 @@ def test_grad_row_counts_around_the_digits_of_the_sort(rows):
     _grad([_randn(53, 400, 9)], [ids], rows, torch.float32)
 
 
-@pytest.mark.parametrize("tokens", [4097, 5100] + ([] if gpu_util.EMULATED else [16384, 16385, 40000]))
+@pytest.mark.parametrize("tokens", [1500, 1501] + ([] if gpu_util.EMULATED else [4096, 4097, 16384, 16385, 65536, 65537]))
 def test_grad_sorts_by_one_workgroup_and_over_several_tiles(tokens):
-    # 4096 and 16384 tokens are the limits of a workgroup's two ways (the host build has its second one at 5000)
+    # one workgroup sorts up to 4096 tokens (up to 1500 in the host build); tiles are of 512, 1024 and 4096
     ids = _ids(54, tokens, 0, 1500)
     _grad([_randn(55, tokens, 8)], [ids], 1500, torch.float32, accumulate=tokens % 2 == 0)
 
