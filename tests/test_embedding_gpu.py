@@ -414,3 +414,46 @@ def test_refusals_of_the_python_layer():
         dfccl_amd.embedding_grad(out, ids, t, workspace=torch.empty(16, dtype=torch.uint8, device=d))
     _sync()
     assert not bool(out.any()) and not bool(t.any())
+
+
+@big_only
+def test_gradients_on_two_streams_at_once():
+    import dfccl_amd
+    s = [torch.cuda.Stream() for _ in range(2)]
+    g = [_randn(90 + k, 9000, 256, dtype=torch.bfloat16) for k in range(2)]
+    ids = [_ids(92 + k, 9000, 0, 700) for k in range(2)]
+    outs = [[torch.empty(700, 256, device="cuda:0") for _ in range(8)] for _ in range(2)]
+    torch.cuda.synchronize()
+    for i in range(8):
+        for k in range(2):
+            dfccl_amd.embedding_grad(g[k], ids[k], outs[k][i], stream=s[k])
+    torch.cuda.synchronize()
+    for k in range(2):
+        exact, before, _ = iu.grad([g[k]], [ids[k]], 700, 0, 1.0, None)
+        iu.check(outs[k][0], exact, before)
+        assert all(torch.equal(outs[k][0], o) for o in outs[k])
+
+
+@big_only
+def test_two_graphs_that_share_a_workspace_replayed_in_turn():
+    import dfccl_amd
+    n = dfccl_amd.embedding_grad_workspace([5000], 400, 96)
+    assert n >= dfccl_amd.embedding_grad_workspace([300], 400, 96)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda:0")
+    g = [_randn(94, 5000, 96), _randn(95, 300, 96)]
+    ids = [_ids(96, 5000, 0, 400), _ids(97, 300, 0, 400)]
+    outs, graphs = [torch.empty(400, 96, device="cuda:0") for _ in range(2)], []
+    torch.cuda.synchronize()
+    for k in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[k]):
+            dfccl_amd.embedding_grad(g[k], ids[k], outs[k], workspace=ws)
+    for turn in range(4):
+        for k in (turn % 2, 1 - turn % 2):
+            ids[k].copy_(_ids(100 + 2 * turn + k, ids[k].numel(), 0, 400))
+            outs[k].fill_(float("nan"))
+            graphs[k].replay()
+        torch.cuda.synchronize()
+        for k in range(2):
+            exact, before, _ = iu.grad([g[k]], [ids[k]], 400, 0, 1.0, None)
+            iu.check(outs[k], exact, before)

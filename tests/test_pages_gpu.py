@@ -357,3 +357,46 @@ def test_refusals():
         dfccl_amd.PageCache.empty(pools, 0, 3, 2).compact()
     _sync()
     assert not bool(cache.refcounts.any()) and cache.lengths.tolist() == [0, 0, 0]
+
+
+@big_only
+def test_two_graphs_of_one_cache_replayed_in_turn():
+    both = Both(pages=300, page_tokens=4, sequences=30, per_seq=30, page_bytes=(256,))
+    seqs, lengths, ended, parents, children = _ints(range(10)), _ints([0] * 10), _ints([0, 1]), _ints([4, 5]), _ints([20, 21])
+    torch.cuda.synchronize()
+    grow, shrink = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(grow):
+        both.cache.extend(seqs, lengths)
+        both.cache.fork(parents, children)
+    with torch.cuda.graph(shrink):
+        both.cache.free(ended)
+        both.cache.compact()
+    rs = np.random.RandomState(21)
+    for turn in range(6):
+        now = [int(both.books.lengths[q]) + int(rs.randint(0, 9)) for q in range(10)]
+        gone = rs.permutation(10)[:2].tolist() + []
+        lengths.copy_(_ints(now))
+        children.copy_(_ints([20 + turn, 26]))
+        ended.copy_(_ints(gone))
+        grow.replay()
+        both.books.extend(list(range(10)), now)
+        both.books.fork([4, 5], [20 + turn, 26])
+        both.same(f"grow {turn}")
+        shrink.replay()
+        both.books.free(gone)
+        both.books.compact()
+        both.same(f"shrink {turn}")
+
+
+@big_only
+def test_pages_of_more_than_4_gigabytes():
+    import dfccl_amd
+    size = (1 << 32) + 1025  # one page: its parts are counted behind 32 bits, and the last one is odd
+    pool = torch.zeros(3, size, dtype=torch.uint8, device="cuda:0")
+    marks = torch.tensor([0, 1, (1 << 31) + 5, (1 << 32) - 1, 1 << 32, size - 2, size - 1], device="cuda:0")
+    pool[2, marks] = torch.arange(1, 8, dtype=torch.uint8, device="cuda:0")
+    cache = dfccl_amd.PageCache.empty([pool], 4, 2, 2)
+    cache.copy(_ints([2]), _ints([0]))
+    _sync()
+    assert torch.equal(pool[0, marks], pool[2, marks]) and int(pool[0].count_nonzero()) == 7
+    assert int(pool[1].count_nonzero()) == 0
