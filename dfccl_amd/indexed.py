@@ -134,9 +134,13 @@ def embedding_grad(grads, ids, table_grad, scale=1.0, first_row=0, padding_id=No
     if workspace is None:
         need = ctypes.c_size_t()
         api.check(lib.dfcclEmbeddingGradWorkspace(n, sizes, rows, width, ctypes.byref(need)), "dfcclEmbeddingGradWorkspace")
-        workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
-        if stream is not None and workspace.is_cuda:
-            workspace.record_stream(stream)
+        # From the pool of the stream that the call runs on: a block of another stream's pool may have been freed by a
+        # tensor whose kernels are still queued there, and this stream does not wait for those.
+        if stream is None:
+            workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
+        else:
+            with torch.cuda.stream(stream):
+                workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
     else:
         _on(device, workspace)
     _call(device, lib.dfcclEmbeddingGrad, "dfcclEmbeddingGrad", grad_ptrs, id_ptrs, sizes, n, api.DTYPE_OF[dtype],
