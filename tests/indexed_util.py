@@ -61,7 +61,8 @@ def grad(grads, ids, rows, first, scale, padding, old=None):
 def check(got, exact, before, what=""):
     off = (got.double().cpu() - exact).abs()
     bound = bound_of_rounding(exact, before, got.dtype)
-    bad = off > bound
+    assert bool(torch.isfinite(bound).all()), f"{what}: the definition and its bound are not finite"
+    bad = ~(off <= bound)  # (NaN is within no bound)
     assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} values too far off, the worst by " \
                           f"{float((off / bound).max()):.3g} bounds, first at {bad.nonzero()[0].tolist()}"
 
