@@ -23,6 +23,11 @@ def _stream_of(device, stream):
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def _capturing(stream):
+    with torch.cuda.stream(stream):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _call(device, fn, what, *args):
     """Runs an entry point with `device` as the current one, as a launch on that device's streams needs it."""
     if device.type == "cuda" and device.index != torch.cuda.current_device():
@@ -153,7 +158,12 @@ class PageCache:
     """A rank's cache of pages (dfcclPageCache): `pools` is a list of contiguous tensors [pages, ...] whose pages hold
     `page_tokens` tokens, and refcounts [pages], tables [sequences, pages per sequence] and lengths [sequences] are its
     bookkeeping, int32 tensors that the caller owns (PageCache.empty makes those of an empty cache).  report[0]:
-    requests refused by the last extend or fork; report[1], report[2]: pages moved, pages live at the last compact."""
+    requests refused by the last extend or fork; report[1], report[2]: pages moved, pages live at the last compact.
+
+    The report and a workspace are the cache's own memory, taken on the stream that is current in the constructor; the
+    first call on another stream waits for what the constructor needs of that one.  A graph with captured calls uses
+    them too: keep the cache as long as the graph, and capture once the constructor's stream has got that far
+    (torch.cuda.graph waits for the device)."""
 
     def __init__(self, pools, page_tokens, refcounts, tables, lengths):
         pages, size, device = pools[0].shape[0], pools[0].nbytes, refcounts.device
@@ -183,6 +193,12 @@ class PageCache:
             tables.shape[0], tables.shape[1], api._dev_ptr(refcounts), api._dev_ptr(tables), api._dev_ptr(lengths),
             api._dev_ptr(self.report), api._dev_ptr(self._workspace), need.value)
         self._ref = ctypes.byref(self._struct)
+        # What comes before this place on the constructor's stream may still use the memory, and clears the report.
+        self._made_on, self._joined, self._made = _stream_of(device, None), {}, None
+        if device.type == "cuda":
+            here = torch.cuda.current_stream(device)
+            if not _capturing(here):
+                self._made = here.record_event()
 
     @classmethod
     def empty(cls, pools, page_tokens, sequences, pages_per_sequence):
@@ -191,6 +207,21 @@ class PageCache:
             return torch.full(shape, value, dtype=torch.int32, device=pools[0].device)
         return cls(pools, page_tokens, ints(0, pools[0].shape[0]), ints(-1, sequences, pages_per_sequence),
                    ints(0, sequences))
+
+    def _stream(self, stream):
+        """The stream's handle, for calls that use the cache's own memory. Another stream than the constructor's waits for
+        that one once, and the memory does not return to its pool before that other stream is through with it."""
+        handle = _stream_of(self._device, stream)
+        if handle != self._made_on and handle not in self._joined:
+            if stream is None:
+                stream = torch.cuda.current_stream(self._device)
+            self._workspace.record_stream(stream)
+            self.report.record_stream(stream)
+            if not _capturing(stream):  # (a capture may not wait for an event from before it)
+                if self._made is not None:
+                    stream.wait_event(self._made)
+                self._joined[handle] = stream
+        return handle
 
     def _lists(self, *lists):
         """Addresses of the lists, and their common length."""
@@ -216,12 +247,12 @@ class PageCache:
     def extend(self, sequences, lengths, stream=None):
         """The sequences grow to these lengths; new entries get the lowest free pages."""
         _call(self._device, self._lib.dfcclPagesExtend, "dfcclPagesExtend", self._ref, *self._lists(sequences, lengths),
-              _stream_of(self._device, stream))
+              self._stream(stream))
 
     def fork(self, parents, children, stream=None):
         """The children (empty) become copies of the parents: full pages shared, a last page that is not full copied."""
         _call(self._device, self._lib.dfcclPagesFork, "dfcclPagesFork", self._ref, *self._lists(parents, children),
-              _stream_of(self._device, stream))
+              self._stream(stream))
 
     def free(self, sequences, stream=None):
         """The sequences become empty and give up their pages."""
@@ -230,4 +261,4 @@ class PageCache:
 
     def compact(self, stream=None):
         """Moves pages until the live ones have the lowest numbers; counts and tables follow."""
-        _call(self._device, self._lib.dfcclPagesCompact, "dfcclPagesCompact", self._ref, _stream_of(self._device, stream))
+        _call(self._device, self._lib.dfcclPagesCompact, "dfcclPagesCompact", self._ref, self._stream(stream))

@@ -71,3 +71,101 @@ def test_the_gradients_workspace_comes_from_the_pool_of_the_stream_that_it_runs_
     assert [args[-1] for args in launched] == [2, 1]
     dfccl_amd.embedding_grad(g, ids, out, workspace=torch.zeros(4096, dtype=torch.uint8), stream=other)
     assert len(machine.taken) == 2 and machine.stream.cuda_stream == 1
+
+
+class Buffer:
+    """A tensor on the GPU, as far as PageCache looks at one."""
+
+    def __init__(self, machine, *shape, dtype=torch.int32):
+        self.machine, self.shape, self.dtype, self.device, self.is_cuda = machine, shape, dtype, torch.device("cuda:0"), True
+        self.nbytes, self.recorded = 4 * self.numel(), []
+
+    def numel(self):
+        return torch.Size(self.shape).numel()
+
+    def dim(self):
+        return len(self.shape)
+
+    def data_ptr(self):
+        return 1 << 20  # never followed
+
+    def is_contiguous(self):
+        return True
+
+    def record_stream(self, stream):
+        self.recorded.append(stream)
+
+
+class Gpu(Machine):
+    def __init__(self):
+        super().__init__()
+        self.stream, self.capturing = Stream(1, "cuda:0"), False
+        self.stream.record_event = lambda: "behind what the constructor needs"
+
+
+@pytest.fixture
+def gpu(machine, monkeypatch):
+    m = Gpu()
+    monkeypatch.setattr(indexed._lib, "load", lambda: m)
+    monkeypatch.setattr(torch, "empty", lambda n, **kw: Buffer(m, n))
+    monkeypatch.setattr(torch, "zeros", lambda n, **kw: Buffer(m, n))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: m.stream)
+    monkeypatch.setattr(indexed, "_raw_stream", lambda index: m.stream.cuda_stream)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: m.capturing)
+    return m
+
+
+def _cache(m):
+    return dfccl_amd.PageCache([Buffer(m, 6, 8)], 4, Buffer(m, 6), Buffer(m, 3, 2), Buffer(m, 3))
+
+
+def _calls(m, cache, first=0, **on):
+    """The three calls that use the cache's own memory, beginning with any of them; returns the handles of their streams."""
+    one, handles = Buffer(m, 1), []
+    calls = [lambda: cache.extend(one, one, **on), lambda: cache.fork(one, one, **on), lambda: cache.compact(**on)]
+    for k in range(3):
+        del m.calls[:]
+        calls[(first + k) % 3]()
+        handles.append(m.calls[0][1][-1])
+    return handles
+
+
+# The workspace and the report come from the pool of the stream that is current in the constructor. Another stream has to
+# wait for what that one still does with them, and they may not return to the pool before the other is through with them.
+@pytest.mark.parametrize("first", range(3))
+def test_a_page_caches_own_memory_is_shared_with_the_streams_that_it_is_used_on(gpu, first):
+    cache, other = _cache(gpu), Stream(2, "cuda:0")
+    assert _calls(gpu, cache, first, stream=other) == [2] * 3
+    assert other.waited == ["behind what the constructor needs"]
+    assert cache._workspace.recorded == [other] and cache.report.recorded == [other]
+    third = Stream(3, "cuda:0")  # not named, but current
+    gpu.stream, made_on = third, gpu.stream
+    assert _calls(gpu, cache, first) == [3] * 3
+    assert third.waited == ["behind what the constructor needs"] and cache.report.recorded == [other, third]
+    gpu.stream = made_on
+    assert _calls(gpu, cache, first) == [1] * 3
+    assert made_on.waited == [] and cache.report.recorded == [other, third]
+
+
+def test_copy_and_free_use_none_of_it_and_wait_for_nothing(gpu):
+    cache, other, one = _cache(gpu), Stream(2, "cuda:0"), Buffer(gpu, 1)
+    cache.copy(one, one, stream=other)
+    cache.free(one, stream=other)
+    assert [args[-1] for _, args in gpu.calls[-2:]] == [2, 2]
+    assert other.waited == [] and cache._workspace.recorded == [] and cache.report.recorded == []
+
+
+def test_a_captured_call_waits_for_no_event_from_before_the_capture(gpu):
+    cache, other = _cache(gpu), Stream(2, "cuda:0")
+    gpu.capturing = True
+    _calls(gpu, cache, stream=other)
+    assert other.waited == [] and set(cache._workspace.recorded) == {other}
+    gpu.capturing = False
+    _calls(gpu, cache, stream=other)
+    assert other.waited == ["behind what the constructor needs"]
+    gpu.capturing = True
+    made_in_a_capture, fourth = _cache(gpu), Stream(4, "cuda:0")  # its memory is the graph's
+    gpu.capturing = False
+    _calls(gpu, made_in_a_capture, stream=fourth)
+    assert fourth.waited == [] and made_in_a_capture.report.recorded == [fourth]
