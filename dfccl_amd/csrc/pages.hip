@@ -31,6 +31,12 @@ constexpr int kScanTile = kScanThreads * kScanPer;
 constexpr int kOneScan = 4;
 constexpr int kFewRequests = 64;  // of an extend, carried out by the workgroup that scans: four for each of its waves, one
                                   // launch less (15 us for a turn of 16 sequences instead of 19)
+// A workgroup per request, up to so many workgroups (a launch may not have 2^32 threads); more requests are walked. (A
+// host build sets a lower limit, to get there with few requests.)
+#ifndef DFCCL_REQUEST_GRID
+#define DFCCL_REQUEST_GRID (1 << 20)
+#endif
+constexpr uint32_t kMaxRequestGrid = DFCCL_REQUEST_GRID;
 
 // The bookkeeping as the kernels see it.
 struct Books {
@@ -189,7 +195,8 @@ __device__ __forceinline__ void extendOne(const Books& b, const PageScratch& s, 
   if (thread == 0) b.lengths[seq] = length;
 }
 __global__ __launch_bounds__(kMoveThreads) void extendKernel(Books b, PageScratch s, Requests q) {
-  extendOne(b, s, q, (int32_t)blockIdx.x, s.counts[0], (int32_t)threadIdx.x, kMoveThreads);
+  for (uint32_t i = blockIdx.x; i < (uint32_t)q.n; i += gridDim.x)
+    extendOne(b, s, q, (int32_t)i, s.counts[0], (int32_t)threadIdx.x, kMoveThreads);
 }
 
 // A few tiles of pages: requests and free pages in one launch, and an extend of a few sequences as a whole.
@@ -331,34 +338,36 @@ __global__ __launch_bounds__(kMoveThreads) void copyKernel(PoolSet p, const int3
 
 // 512 forks of 8 pools' 16 KiB pages: 16 children read the same page, so loads stay in the caches (25 us for the call; 39
 // if they do not). Two loads a lane: 25 us, four 27, one 33 (every wave looks its request up).
-// Fork. The first q.n workgroups (of the first launch, if the pools take several) write the tables, one per request:
-// the child's whole pages are the parent's, a last page that is not full is the child's own. The others copy the
-// contents of those. Neither reads what the other writes: children were empty, and parents stay as they are.
+// Fork. The first tableBlocks workgroups (of the first launch, if the pools take several) write the tables: a child's
+// whole pages are the parent's, a last page that is not full is the child's own. The others copy the contents of those.
+// Neither reads what the other writes: children were empty, and parents stay as they are.
+__device__ __forceinline__ void forkOne(const Books& b, const PageScratch& s, const Requests& q, uint32_t i) {
+  const int32_t first = s.request[i], before = s.before[i];
+  const int32_t whole = before / b.pageTokens, need = before % b.pageTokens != 0;
+  if (first < 0 || (need != 0 && first >= s.counts[0])) {
+    if (threadIdx.x == 0) refuse(b);
+    return;
+  }
+  const int32_t parent = q.a[i], child = q.b[i];
+  const int32_t* from = b.tables + (size_t)parent * b.perSeq;
+  int32_t* to = b.tables + (size_t)child * b.perSeq;
+  for (int32_t k = (int32_t)threadIdx.x; k < whole; k += kMoveThreads) {
+    const int32_t page = from[k];
+    to[k] = page;
+    if (page >= 0 && page < b.pages) __hip_atomic_fetch_add(&b.refcounts[page], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if (threadIdx.x == 0) {
+    if (need != 0) {
+      const int32_t page = s.found[first];
+      to[whole] = page;
+      b.refcounts[page] = 1;
+    }
+    b.lengths[child] = before;
+  }
+}
 __global__ __launch_bounds__(kMoveThreads) void forkKernel(Books b, PageScratch s, Requests q, PoolSet p, uint32_t tableBlocks) {
   if (blockIdx.x < tableBlocks) {
-    const int32_t i = (int32_t)blockIdx.x;
-    const int32_t first = s.request[i], before = s.before[i];
-    const int32_t whole = before / b.pageTokens, need = before % b.pageTokens != 0;
-    if (first < 0 || (need != 0 && first >= s.counts[0])) {
-      if (threadIdx.x == 0) refuse(b);
-      return;
-    }
-    const int32_t parent = q.a[i], child = q.b[i];
-    const int32_t* from = b.tables + (size_t)parent * b.perSeq;
-    int32_t* to = b.tables + (size_t)child * b.perSeq;
-    for (int32_t k = (int32_t)threadIdx.x; k < whole; k += kMoveThreads) {
-      const int32_t page = from[k];
-      to[k] = page;
-      if (page >= 0 && page < b.pages) __hip_atomic_fetch_add(&b.refcounts[page], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    if (threadIdx.x == 0) {
-      if (need != 0) {
-        const int32_t page = s.found[first];
-        to[whole] = page;
-        b.refcounts[page] = 1;
-      }
-      b.lengths[child] = before;
-    }
+    for (uint32_t i = blockIdx.x; i < (uint32_t)q.n; i += tableBlocks) forkOne(b, s, q, i);
     return;
   }
   const int lane = (int)(threadIdx.x & 63);
@@ -625,6 +634,7 @@ constexpr unsigned kMaxCompactGrid = 1u << 16;
 static unsigned moveGrid(uint64_t items) {
   return (unsigned)std::max<uint64_t>(1, std::min<uint64_t>((items + kMoveWaves - 1) / kMoveWaves, kMaxMoveGrid));
 }
+static unsigned requestGrid(int n) { return std::min((uint32_t)n, kMaxRequestGrid); }
 // Returns whether that has carried the requests out, too.
 template <int FOR>
 static bool launchAssign(const Books& b, const PageScratch& s, const Requests& q, hipStream_t st) {
@@ -678,7 +688,7 @@ DFCCL_API ncclResult_t dfcclPagesExtend(const dfcclPageCache* c, const int32_t* 
   const PageScratch s = scratchOf(c);
   const Requests q{sequences, lengths, n};
   const bool done = launchAssign<kForExtend>(b, s, q, st);
-  if (n > 0 && !done) DFCCL_LAUNCH_BLOCKS(extendKernel, (unsigned)n, kMoveThreads, st, b, s, q);
+  if (n > 0 && !done) DFCCL_LAUNCH_BLOCKS(extendKernel, requestGrid(n), kMoveThreads, st, b, s, q);
   return launched();
 }
 
@@ -693,7 +703,7 @@ DFCCL_API ncclResult_t dfcclPagesFork(const dfcclPageCache* c, const int32_t* pa
   (void)launchAssign<kForFork>(b, s, q, st);
   for (int first = 0; n > 0 && first < c->npools; first += kMaxPools) {
     const PoolSet p = poolSet(c, c, first, kForkLoads);
-    const unsigned tableBlocks = first == 0 ? (unsigned)n : 0u;
+    const unsigned tableBlocks = first == 0 ? requestGrid(n) : 0u;
     DFCCL_LAUNCH_BLOCKS(forkKernel, tableBlocks + moveGrid((uint64_t)n * p.npools * p.parts), kMoveThreads, st, b, s, q, p,
                         tableBlocks);
   }
@@ -703,7 +713,7 @@ DFCCL_API ncclResult_t dfcclPagesFork(const dfcclPageCache* c, const int32_t* pa
 DFCCL_API ncclResult_t dfcclPagesFree(const dfcclPageCache* c, const int32_t* sequences, int n, void* stream) {
   if (!soundCache(c) || n < 0 || (n > 0 && sequences == nullptr)) return ncclInvalidArgument;
   if (n == 0) return ncclSuccess;
-  DFCCL_LAUNCH_BLOCKS(freeKernel, (unsigned)std::min(n, 1 << 20), kMoveThreads, (hipStream_t)stream, booksOf(c), sequences, n);
+  DFCCL_LAUNCH_BLOCKS(freeKernel, requestGrid(n), kMoveThreads, (hipStream_t)stream, booksOf(c), sequences, n);
   return launched();
 }
 

@@ -153,7 +153,15 @@ void launch(Stream* s, unsigned grid, unsigned block, std::function<void()> body
   gJobs.push_back(job);
 }
 
+// threads that a launch may have; a GPU refuses 2^32
+static std::atomic<uint64_t> gLaunchLimit{(1ull << 32) - 1};
+static thread_local hipError_t gLastError = hipSuccess;
+
 void launchBlocks(Stream* s, unsigned grid, unsigned block, std::function<void()> body) {
+  if ((uint64_t)grid * block > gLaunchLimit.load()) {
+    gLastError = hipErrorInvalidConfiguration;
+    return;
+  }
   if (s == nullptr) s = &gNullStream;
   std::shared_ptr<Job> prev;
   {
@@ -242,6 +250,7 @@ static void startWatchdog() {
 
 }  // namespace emul
 
+extern "C" void emulLaunchLimit(uint64_t threads) { emul::gLaunchLimit.store(threads); }
 extern "C" void emulDumpThreads() { emul::dumpThreads(stderr); }
 // for callers outside C++ (the Python tests): wait for the kernels launched on the null stream
 extern "C" void emulNullStreamSynchronize() { (void)hipStreamSynchronize(nullptr); }
@@ -291,7 +300,11 @@ hipError_t hipDeviceGetAttribute(int* value, hipDeviceAttribute_t, int) {
   *value = 256;
   return hipSuccess;
 }
-hipError_t hipGetLastError() { return hipSuccess; }
+hipError_t hipGetLastError() {
+  const hipError_t e = emul::gLastError;
+  emul::gLastError = hipSuccess;
+  return e;
+}
 const char* hipGetErrorString(hipError_t e) { return e == hipSuccess ? "no error" : "emulated error"; }
 hipError_t hipStreamCreateWithFlags(hipStream_t* s, unsigned) {
   *s = new emul::Stream();

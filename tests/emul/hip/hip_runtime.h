@@ -213,7 +213,7 @@ inline float __uint_as_float(uint32_t u) { return __builtin_bit_cast(float, u); 
 
 // ---- runtime API (the part the library and its native driver use)
 typedef int hipError_t;
-enum : int { hipSuccess = 0, hipErrorInvalidValue = 1, hipErrorOutOfMemory = 2, hipErrorNotReady = 600 };
+enum : int { hipSuccess = 0, hipErrorInvalidValue = 1, hipErrorOutOfMemory = 2, hipErrorInvalidConfiguration = 9, hipErrorNotReady = 600 };
 typedef emul::Stream* hipStream_t;
 typedef emul::Event* hipEvent_t;
 typedef void* hipDeviceptr_t;
