@@ -37,6 +37,8 @@ constexpr int kFewRequests = 64;  // of an extend, carried out by the workgroup 
 #define DFCCL_REQUEST_GRID (1 << 20)
 #endif
 constexpr uint32_t kMaxRequestGrid = DFCCL_REQUEST_GRID;
+// Counter of a walk over a list, the sequences or a table row: its last step goes beyond the last of up to 2^31 - 1 entries.
+using ListIndex = uint32_t;
 
 // The bookkeeping as the kernels see it.
 struct Books {
@@ -121,30 +123,30 @@ struct Requests {
 // One workgroup; returns the pages that all of them need.
 template <bool FORK>
 __device__ __forceinline__ int32_t readRequests(ScanShared& sh, const Books& b, const PageScratch& s, const Requests& q) {
-  const int tid = (int)threadIdx.x;
+  const ListIndex tid = threadIdx.x, n = (ListIndex)q.n;
   const int64_t most = (int64_t)b.perSeq * b.pageTokens;
   // the first request that names a sequence (a fork: a child) has it; the others are refused
-  for (int32_t i = tid; i < q.n; i += kScanThreads) {
+  for (ListIndex i = tid; i < n; i += kScanThreads) {
     const int32_t seq = FORK ? q.b[i] : q.a[i];
     if (seq >= 0 && seq < b.seqs) s.owner[seq] = 0x7fffffff;
   }
   __syncthreads();
-  for (int32_t i = tid; i < q.n; i += kScanThreads) {
+  for (ListIndex i = tid; i < n; i += kScanThreads) {
     const int32_t seq = FORK ? q.b[i] : q.a[i];
     if (seq >= 0 && seq < b.seqs)
-      __hip_atomic_fetch_min(&s.owner[seq], i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_fetch_min(&s.owner[seq], (int32_t)i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
   int32_t needed = 0;  // (at most seqs * perSeq, which the host keeps below 2^31)
   int which = 0;
-  for (int32_t at = 0; at < q.n; at += kScanThreads, which ^= 1) {
-    const int32_t i = at + tid;
+  for (ListIndex at = 0; at < n; at += kScanThreads, which ^= 1) {
+    const ListIndex i = at + tid;
     int32_t need = -1, before = 0;
-    if (i < q.n) {
+    if (i < n) {
       const int32_t x = q.a[i], y = q.b[i];
       const int32_t seq = FORK ? y : x;
       if (seq >= 0 && seq < b.seqs && x >= 0 && x < b.seqs &&
-          __hip_atomic_load(&s.owner[seq], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == i) {
+          __hip_atomic_load(&s.owner[seq], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int32_t)i) {
         before = b.lengths[x];
         const bool sound = before >= 0 && before <= most;
         if constexpr (FORK) {
@@ -157,7 +159,7 @@ __device__ __forceinline__ int32_t readRequests(ScanShared& sh, const Books& b, 
     }
     int32_t total;
     const int32_t first = blockScan(sh, which, need > 0 ? need : 0, total);
-    if (i < q.n) s.request[i] = need < 0 ? -1 : needed + first;
+    if (i < n) s.request[i] = need < 0 ? -1 : needed + first;
     needed += total;
   }
   __syncthreads();
@@ -170,8 +172,8 @@ __device__ __forceinline__ void refuse(const Books& b) {
 }
 
 // One request of an extend, by `threads` threads: the new entries, their counts, the length.
-__device__ __forceinline__ void extendOne(const Books& b, const PageScratch& s, const Requests& q, int32_t i, int32_t foundPages,
-                                          int32_t thread, int32_t threads) {
+__device__ __forceinline__ void extendOne(const Books& b, const PageScratch& s, const Requests& q, ListIndex i, int32_t foundPages,
+                                          uint32_t thread, uint32_t threads) {
   const int32_t first = s.request[i];
   int32_t have = 0, want = 0, seq = 0, length = 0;
   bool met = false;
@@ -187,16 +189,16 @@ __device__ __forceinline__ void extendOne(const Books& b, const PageScratch& s, 
     return;
   }
   int32_t* row = b.tables + (size_t)seq * b.perSeq;
-  for (int32_t k = have + thread; k < want; k += threads) {
-    const int32_t page = s.found[first + k - have];
+  for (ListIndex k = (ListIndex)have + thread; k < (ListIndex)want; k += threads) {
+    const int32_t page = s.found[(ListIndex)first + (k - (ListIndex)have)];
     row[k] = page;
     b.refcounts[page] = 1;
   }
   if (thread == 0) b.lengths[seq] = length;
 }
 __global__ __launch_bounds__(kMoveThreads) void extendKernel(Books b, PageScratch s, Requests q) {
-  for (uint32_t i = blockIdx.x; i < (uint32_t)q.n; i += gridDim.x)
-    extendOne(b, s, q, (int32_t)i, s.counts[0], (int32_t)threadIdx.x, kMoveThreads);
+  for (ListIndex i = blockIdx.x; i < (ListIndex)q.n; i += gridDim.x)
+    extendOne(b, s, q, i, s.counts[0], threadIdx.x, kMoveThreads);
 }
 
 // A few tiles of pages: requests and free pages in one launch, and an extend of a few sequences as a whole.
@@ -216,7 +218,8 @@ __global__ __launch_bounds__(kScanThreads) void assignKernel(Books b, PageScratc
   if constexpr (!FORK) {
     if (!carryOut) return;
     __syncthreads();
-    for (int32_t i = waveInBlock(); i < q.n; i += kScanWaves) extendOne(b, s, q, i, foundPages, (int32_t)(threadIdx.x & 63), 64);
+    for (ListIndex i = (ListIndex)waveInBlock(); i < (ListIndex)q.n; i += kScanWaves)
+      extendOne(b, s, q, i, foundPages, threadIdx.x & 63, 64);
   }
 }
 
@@ -248,7 +251,7 @@ __global__ __launch_bounds__(kScanThreads) void countTilesKernel(Books b, PageSc
 // The sum of the first n tiles' counts, by the workgroup.
 __device__ __forceinline__ int32_t sumTiles(ScanShared& sh, int which, const int32_t* tiles, int32_t n) {
   int32_t mine = 0, total;
-  for (int32_t t = (int32_t)threadIdx.x; t < n; t += kScanThreads) mine += tiles[t];
+  for (uint32_t t = threadIdx.x; t < (uint32_t)n; t += kScanThreads) mine += tiles[t];
   (void)blockScan(sh, which, mine, total);
   return total;
 }
@@ -341,7 +344,7 @@ __global__ __launch_bounds__(kMoveThreads) void copyKernel(PoolSet p, const int3
 // Fork. The first tableBlocks workgroups (of the first launch, if the pools take several) write the tables: a child's
 // whole pages are the parent's, a last page that is not full is the child's own. The others copy the contents of those.
 // Neither reads what the other writes: children were empty, and parents stay as they are.
-__device__ __forceinline__ void forkOne(const Books& b, const PageScratch& s, const Requests& q, uint32_t i) {
+__device__ __forceinline__ void forkOne(const Books& b, const PageScratch& s, const Requests& q, ListIndex i) {
   const int32_t first = s.request[i], before = s.before[i];
   const int32_t whole = before / b.pageTokens, need = before % b.pageTokens != 0;
   if (first < 0 || (need != 0 && first >= s.counts[0])) {
@@ -351,7 +354,7 @@ __device__ __forceinline__ void forkOne(const Books& b, const PageScratch& s, co
   const int32_t parent = q.a[i], child = q.b[i];
   const int32_t* from = b.tables + (size_t)parent * b.perSeq;
   int32_t* to = b.tables + (size_t)child * b.perSeq;
-  for (int32_t k = (int32_t)threadIdx.x; k < whole; k += kMoveThreads) {
+  for (ListIndex k = threadIdx.x; k < (ListIndex)whole; k += kMoveThreads) {
     const int32_t page = from[k];
     to[k] = page;
     if (page >= 0 && page < b.pages) __hip_atomic_fetch_add(&b.refcounts[page], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -367,7 +370,7 @@ __device__ __forceinline__ void forkOne(const Books& b, const PageScratch& s, co
 }
 __global__ __launch_bounds__(kMoveThreads) void forkKernel(Books b, PageScratch s, Requests q, PoolSet p, uint32_t tableBlocks) {
   if (blockIdx.x < tableBlocks) {
-    for (uint32_t i = blockIdx.x; i < (uint32_t)q.n; i += tableBlocks) forkOne(b, s, q, i);
+    for (ListIndex i = blockIdx.x; i < (ListIndex)q.n; i += tableBlocks) forkOne(b, s, q, i);
     return;
   }
   const int lane = (int)(threadIdx.x & 63);
@@ -390,7 +393,7 @@ __global__ __launch_bounds__(kMoveThreads) void freeKernel(Books b, const int32_
     int32_t length;
   };
   DFCCL_WG_SHARED(Shared, sh);
-  for (int32_t i = (int32_t)blockIdx.x; i < n; i += (int32_t)gridDim.x) {
+  for (ListIndex i = blockIdx.x; i < (ListIndex)n; i += gridDim.x) {
     const int32_t seq = seqs[i];
     if (threadIdx.x == 0)
       sh.length = seq >= 0 && seq < b.seqs
@@ -402,7 +405,7 @@ __global__ __launch_bounds__(kMoveThreads) void freeKernel(Books b, const int32_
       int32_t used = pagesOf(length, b.pageTokens);
       if (used > b.perSeq) used = b.perSeq;
       int32_t* row = b.tables + (size_t)seq * b.perSeq;
-      for (int32_t k = (int32_t)threadIdx.x; k < used; k += kMoveThreads) {
+      for (ListIndex k = threadIdx.x; k < (ListIndex)used; k += kMoveThreads) {
         const int32_t page = row[k];
         row[k] = -1;
         if (page >= 0 && page < b.pages)
@@ -520,18 +523,18 @@ __global__ __launch_bounds__(kScanThreads) void listMovesKernel(Books b, PageScr
 __global__ __launch_bounds__(kMoveThreads) void compactKernel(Books b, PageScratch s, PoolSet p, uint32_t bookBlocks) {
   const int32_t moves = uniform(s.counts[1]);
   if (blockIdx.x < bookBlocks) {
-    for (int32_t i = (int32_t)(blockIdx.x * kMoveThreads + threadIdx.x); i < moves; i += (int32_t)(bookBlocks * kMoveThreads)) {
+    for (ListIndex i = blockIdx.x * kMoveThreads + threadIdx.x; i < (ListIndex)moves; i += bookBlocks * kMoveThreads) {
       const int32_t from = s.movers[i], to = s.found[i];
       b.refcounts[to] = b.refcounts[from];
       b.refcounts[from] = 0;
     }
-    for (int32_t seq = (int32_t)blockIdx.x; seq < b.seqs; seq += (int32_t)bookBlocks) {
+    for (ListIndex seq = blockIdx.x; seq < (ListIndex)b.seqs; seq += bookBlocks) {
       const int32_t length = b.lengths[seq];
       if (length <= 0) continue;
       int32_t used = pagesOf(length, b.pageTokens);
       if (used > b.perSeq) used = b.perSeq;
       int32_t* row = b.tables + (size_t)seq * b.perSeq;
-      for (int32_t k = (int32_t)threadIdx.x; k < used; k += kMoveThreads) {
+      for (ListIndex k = threadIdx.x; k < (ListIndex)used; k += kMoveThreads) {
         const int32_t page = row[k];
         if (page < 0 || page >= b.pages) continue;
         const int32_t r = s.rank[page];  // (left over from anywhere for a page that does not move)
@@ -629,6 +632,7 @@ static PoolSet poolSet(const dfcclPageCache* to, const dfcclPageCache* from, int
   p.lastBytes = (uint32_t)(to->pageBytes - (size_t)(p.parts - 1) * partBytes(loads));
   return p;
 }
+static_assert(0x7fffffffull + kMaxRequestGrid <= (ListIndex)~0u, "a walk's last step");
 constexpr uint64_t kMaxMoveGrid = 1u << 22;
 constexpr unsigned kMaxCompactGrid = 1u << 16;
 static unsigned moveGrid(uint64_t items) {

@@ -69,3 +69,13 @@ def test_extend_and_fork_of_more_requests_than_a_grid_has_workgroups(limited):
     cache.call("Fork", rs.randint(-1, 201, 199), 200 + rs.permutation(199))  # (refusals and shared parents among them)
     cache.call("Extend", rs.permutation(400), rs.randint(0, 26, 400))
     cache.call("Free", rs.permutation(400)[:250])
+
+
+def test_no_walk_over_a_list_counts_in_a_type_that_its_last_step_leaves():
+    # lists, sequences and table rows have up to 2^31 - 1 entries, and a walk's last step goes beyond the last one by up
+    # to a grid: with a signed counter of 32 bits it would come out negative, and be followed
+    import re
+    with open(os.path.join(ROOT, "dfccl_amd", "csrc", "pages.hip")) as f:
+        walks = re.findall(r"for \((\w+) (\w+) = [^;]*; ([^;]*); \2 \+= [^)]*", f.read())
+    kinds = {kind for kind, _, end in walks if "npools" not in end}
+    assert len(walks) >= 15 and kinds <= {"int64_t", "uint64_t", "uint32_t", "ListIndex"}
