@@ -78,6 +78,13 @@ def _on(device, *tensors):
             raise ValueError(f"tensors on {device} and {t.device}: one call works on one device")
 
 
+def _fits(bits, what, *numbers):
+    """Refuses what ctypes would pass on as another number: it drops the bits that the C type does not hold."""
+    for n in numbers:
+        if not -1 << bits - 1 <= n < 1 << bits - 1:
+            raise ValueError(f"{what}: {n} does not fit {bits} bits")
+
+
 def embedding_lookup(table, ids, out, scale=1.0, first_row=0, stream=None):
     """out[t, :] = scale * table[ids[t] - first_row, :] (dfcclEmbeddingLookup), zeros for ids outside the table, which
     may be one rank's piece of the vocabulary.  ids may have any shape, out is [ids.numel(), width]; rows of `table`
@@ -89,6 +96,7 @@ def embedding_lookup(table, ids, out, scale=1.0, first_row=0, stream=None):
     if tuple(out.shape) != (tokens, width):
         raise ValueError(f"out has shape {tuple(out.shape)}, not {(tokens, width)}")
     _on(device, out)
+    _fits(64, "first_row", first_row)
     _call(device, _lib.load().dfcclEmbeddingLookup, "dfcclEmbeddingLookup", table_ptr, api.DTYPE_OF[table.dtype], rows,
           table_stride, first_row, _ids_ptr(ids, device), api.DTYPE_OF[ids.dtype], tokens, width, scale, out_ptr,
           api.DTYPE_OF[out.dtype], out_stride, _stream_of(device, stream))
@@ -97,6 +105,7 @@ def embedding_lookup(table, ids, out, scale=1.0, first_row=0, stream=None):
 def embedding_grad_workspace(tokens, rows, width):
     """Bytes of workspace that embedding_grad needs for sources of so many tokens (a list)."""
     n = ctypes.c_size_t()
+    _fits(64, "sizes", *tokens, rows, width)
     api.check(_lib.load().dfcclEmbeddingGradWorkspace(len(tokens), (ctypes.c_size_t * len(tokens))(*tokens), rows, width,
                                                       ctypes.byref(n)), "dfcclEmbeddingGradWorkspace")
     return n.value
@@ -118,6 +127,9 @@ def embedding_grad(grads, ids, table_grad, scale=1.0, first_row=0, padding_id=No
     device, dtype, id_type = table_grad.device, grads[0].dtype, ids[0].dtype
     if dtype not in _FLOATS:
         raise TypeError(f"grads: dtype {dtype} is not one of float32, float16, bfloat16")
+    _fits(64, "first_row", first_row)
+    padding_id = -1 if padding_id is None else padding_id
+    _fits(64, "padding_id", padding_id)
     grad_ptrs, id_ptrs, sizes = (ctypes.c_void_p * n)(), (ctypes.c_void_p * n)(), (ctypes.c_size_t * n)()
     grad_stride = None
     for r in range(n):
@@ -150,7 +162,7 @@ def embedding_grad(grads, ids, table_grad, scale=1.0, first_row=0, padding_id=No
         _on(device, workspace)
     _call(device, lib.dfcclEmbeddingGrad, "dfcclEmbeddingGrad", grad_ptrs, id_ptrs, sizes, n, api.DTYPE_OF[dtype],
           width if grad_stride is None else grad_stride, api.DTYPE_OF[id_type], first_row, rows, width,
-          -1 if padding_id is None else padding_id, scale, int(accumulate), table_ptr, api.DTYPE_OF[table_grad.dtype],
+          padding_id, scale, int(accumulate), table_ptr, api.DTYPE_OF[table_grad.dtype],
           table_stride, api._dev_ptr(workspace), workspace.numel() * workspace.element_size(), _stream_of(device, stream))
 
 
@@ -180,6 +192,7 @@ class PageCache:
         if refcounts.shape != (pages,) or tables.dim() != 2 or lengths.shape != (tables.shape[0],):
             raise ValueError("refcounts is [pages], tables [sequences, pages per sequence], lengths [sequences]")
         _on(device, tables, lengths)
+        _fits(32, "a cache's sizes", len(pools), pages, page_tokens, *tables.shape)
         lib = _lib.load()
         need = ctypes.c_size_t()
         api.check(lib.dfcclPageCacheWorkspace(pages, tables.shape[0], ctypes.byref(need)), "dfcclPageCacheWorkspace")
@@ -226,6 +239,7 @@ class PageCache:
     def _lists(self, *lists):
         """Addresses of the lists, and their common length."""
         n = lists[0].numel()
+        _fits(32, "a list's length", n)
         for t in lists:
             if t.dtype is not torch.int32:
                 raise TypeError("lists of sequences, pages and lengths are int32 tensors")

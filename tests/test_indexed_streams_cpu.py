@@ -169,3 +169,42 @@ def test_a_captured_call_waits_for_no_event_from_before_the_capture(gpu):
     gpu.capturing = False
     _calls(gpu, made_in_a_capture, stream=fourth)
     assert fourth.waited == [] and made_in_a_capture.report.recorded == [fourth]
+
+
+# ctypes drops the bits of an integer that its C type does not hold: what would arrive as another number is refused
+@pytest.mark.parametrize("number", [1 << 63, -(1 << 63) - 1, 1 << 64, (1 << 64) + 3])
+def test_ids_that_do_not_fit_64_bits_are_refused(machine, number):
+    table, ids, out = torch.zeros(5, 8), torch.zeros(3, dtype=torch.int64), torch.zeros(3, 8)
+    with pytest.raises(ValueError, match="first_row.* 64 bits"):
+        dfccl_amd.embedding_lookup(table, ids, out, first_row=number)
+    with pytest.raises(ValueError, match="first_row.* 64 bits"):
+        dfccl_amd.embedding_grad(out, ids, table, first_row=number)
+    with pytest.raises(ValueError, match="padding_id.* 64 bits"):
+        dfccl_amd.embedding_grad(out, ids, table, padding_id=number)
+    with pytest.raises(ValueError, match="64 bits"):
+        dfccl_amd.embedding_grad_workspace([3], number, 8)
+    assert not [name for name, _ in machine.calls if not name.endswith("Workspace")]
+    for fits in ((1 << 63) - 1, -(1 << 63)):
+        dfccl_amd.embedding_lookup(table, ids, out, first_row=fits)
+        dfccl_amd.embedding_grad(out, ids, table, first_row=fits, padding_id=fits)
+    assert len([name for name, _ in machine.calls if not name.endswith("Workspace")]) == 4
+
+
+@pytest.mark.parametrize("number", [1 << 31, 1 << 32, (1 << 32) + 4, -(1 << 31) - 1])
+def test_sizes_of_a_page_cache_that_do_not_fit_32_bits_are_refused(gpu, number):
+    def make(pages=6, page_tokens=4, sequences=3, per_seq=2):
+        return dfccl_amd.PageCache([Buffer(gpu, pages, 8)], page_tokens, Buffer(gpu, pages), Buffer(gpu, sequences, per_seq),
+                                   Buffer(gpu, sequences))
+    with pytest.raises(ValueError, match="32 bits"):
+        make(page_tokens=number)
+    if number > 0:
+        for size in ("pages", "sequences", "per_seq"):
+            with pytest.raises(ValueError, match="32 bits"):
+                make(**{size: number})
+        cache, many = make(), Buffer(gpu, number)
+        del gpu.calls[:]
+        for call in (lambda: cache.free(many), lambda: cache.copy(many, many), lambda: cache.extend(many, many),
+                     lambda: cache.fork(many, many)):
+            with pytest.raises(ValueError, match="32 bits"):
+                call()
+        assert not gpu.calls
