@@ -17,6 +17,8 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the curren
 
 def _stream_of(device, stream):
     if stream is not None:
+        if stream.device != device:
+            raise ValueError(f"tensors on {device}, stream on {stream.device}: one call works on one device")
         return stream.cuda_stream
     if device.type == "cuda" and _raw_stream is not None:
         return _raw_stream(device.index)
@@ -147,7 +149,7 @@ def embedding_grad(grads, ids, table_grad, scale=1.0, first_row=0, padding_id=No
             if grad_stride is not None and grad_stride != stride:
                 raise ValueError("the sources must agree in their row stride")
             grad_stride = stride
-    lib = _lib.load()
+    lib, handle = _lib.load(), _stream_of(device, stream)
     if workspace is None:
         need = ctypes.c_size_t()
         api.check(lib.dfcclEmbeddingGradWorkspace(n, sizes, rows, width, ctypes.byref(need)), "dfcclEmbeddingGradWorkspace")
@@ -163,7 +165,7 @@ def embedding_grad(grads, ids, table_grad, scale=1.0, first_row=0, padding_id=No
     _call(device, lib.dfcclEmbeddingGrad, "dfcclEmbeddingGrad", grad_ptrs, id_ptrs, sizes, n, api.DTYPE_OF[dtype],
           width if grad_stride is None else grad_stride, api.DTYPE_OF[id_type], first_row, rows, width,
           padding_id, scale, int(accumulate), table_ptr, api.DTYPE_OF[table_grad.dtype],
-          table_stride, api._dev_ptr(workspace), workspace.numel() * workspace.element_size(), _stream_of(device, stream))
+          table_stride, api._dev_ptr(workspace), workspace.numel() * workspace.element_size(), handle)
 
 
 class PageCache:

@@ -208,3 +208,24 @@ def test_sizes_of_a_page_cache_that_do_not_fit_32_bits_are_refused(gpu, number):
             with pytest.raises(ValueError, match="32 bits"):
                 call()
         assert not gpu.calls
+
+
+def test_a_stream_of_another_device_is_refused(gpu):
+    elsewhere, one = Stream(2, "cuda:1"), Buffer(gpu, 1)
+    cache = _cache(gpu)
+    del gpu.calls[:]
+    for call in (lambda: cache.copy(one, one, stream=elsewhere), lambda: cache.extend(one, one, stream=elsewhere),
+                 lambda: cache.fork(one, one, stream=elsewhere), lambda: cache.free(one, stream=elsewhere),
+                 lambda: cache.compact(stream=elsewhere)):
+        with pytest.raises(ValueError, match="stream on cuda:1"):
+            call()
+    assert not gpu.calls and not elsewhere.waited and not cache._workspace.recorded
+
+
+def test_a_lookup_and_a_gradient_on_a_stream_of_another_device_are_refused(machine):
+    table, ids, out = torch.zeros(5, 8), torch.zeros(3, dtype=torch.int64), torch.zeros(3, 8)
+    for call in (lambda s: dfccl_amd.embedding_lookup(table, ids, out, stream=s),
+                 lambda s: dfccl_amd.embedding_grad(out, ids, table, stream=s)):
+        with pytest.raises(ValueError, match="stream on cuda:1"):
+            call(Stream(2, "cuda:1"))
+    assert not machine.taken and not [name for name, _ in machine.calls if not name.endswith("Workspace")]
