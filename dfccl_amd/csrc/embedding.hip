@@ -116,7 +116,8 @@ static LookupKernel pickLookup(int in, int out) {
 //
 // 1. Sort. Every token gets a key, its row (or `rows` if it does not count: outside the piece, or padding), and a
 //    payload, its source and number. A radix sort from the low digit up, stable and without atomics on positions,
-//    puts equal keys side by side in the order source, token: the order of every sum is fixed by the ids alone.
+//    puts equal keys side by side in the order source, token: the order of every sum is fixed by the ids and the rows
+//    that they name here (where a block of 2. begins in a run depends on how many tokens the rows before have).
 // 2. Chunks. The sorted list is cut into chunks of kChunk. A chunk that lies within one row's run is summed by a
 //    wave of its own into fp32 scratch, and so are kSuper such chunks: a row that many tokens share (padding that
 //    counts, frequent words) is summed by many waves, and again in a fixed order.

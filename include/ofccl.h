@@ -211,8 +211,11 @@ ncclResult_t dfcclEmbeddingLookup(const void* table, ncclDataType_t tableType, s
 /* tableGrad[v,:] = scale * the sum of grads[r][t,:] over all tokens t of all
  * sources r (1..8: the ranks' batches, tokens[r] < 2^28 each) whose id names
  * row v.  Tokens whose id is paddingId (negative: no such id) are left out.
- * Summed in fp32 in an order that depends on the ids alone (source by source,
- * token by token, long runs in blocks): the same call gives the same bits.
+ * Summed in fp32, source by source, token by token, a row's run of 16 and more
+ * tokens in blocks.  The order depends on the ids and on which of them name
+ * rows, on nothing else: the same call gives the same bits.  Blocks begin
+ * anywhere in a run, so a piece of the vocabulary need not give the bits that
+ * the whole table gives for the same row; both are sums within the same bound.
  * accumulate = 0 writes every row (zeros where no token names one);
  * accumulate = 1 adds to the rows that tokens name and touches no other.
  * grads, ids and tokens are host arrays of nsrcs entries; tokens[r] may be 0.
