@@ -386,9 +386,11 @@ __global__ __launch_bounds__(kSmallThreads) void sortSmallKernel(GradArgs a, int
 // ---- more tokens: tiles, a count and a scatter per digit (4 and 7 us at 13000 tokens, of which the launches are half)
 constexpr int kSortThreads = 256;
 constexpr int kSortWaves = kSortThreads / 64;
-// 64-key strips of a wave of a tile: few enough that the tokens spread over several workgroups, many enough that there
-// are not more than a few dozen histograms, which every tile adds up for itself (2 instead of 4 strips: 40 instead of
-// 42 us for a call on 13000 tokens)
+// 64-key strips of a wave of a tile: few enough that the tokens spread over several workgroups, many enough that there are
+// few histograms, which every tile adds up for itself. Calls that add to 131072 rows of 8 columns (two digits): 16384
+// tokens 35 us with 2 strips and 36 with 4, 24576 tokens 40 and 39; 65536 tokens 56 us with 4 and 68 with 16, 131072
+// tokens 84 with either, 262144 tokens 139 and 119. Beyond, tiles and so histograms grow with the tokens, and what all
+// tiles read of them with the square: 1 M tokens (256 tiles) 0.31 ms, 4 M 1.0 ms, 16 M (4096 tiles) 6.6 ms.
 static int stripsOf(uint64_t n) { return n <= 16u * 1024 ? 2 : n <= 64u * 1024 ? 4 : 16; }
 
 // The keys and payloads of a tile's strips before the first pass, a few strips at a time.

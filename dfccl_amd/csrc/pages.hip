@@ -339,11 +339,7 @@ __global__ __launch_bounds__(kMoveThreads) void copyKernel(PoolSet p, const int3
   }
 }
 
-// 512 forks of 8 pools' 16 KiB pages: 16 children read the same page, so loads stay in the caches (25 us for the call; 39
-// if they do not). Two loads a lane: 25 us, four 27, one 33 (every wave looks its request up).
-// Fork. The first tableBlocks workgroups (of the first launch, if the pools take several) write the tables: a child's
-// whole pages are the parent's, a last page that is not full is the child's own. The others copy the contents of those.
-// Neither reads what the other writes: children were empty, and parents stay as they are.
+// One request of a fork, by a workgroup: the child's whole pages are the parent's, a last page that is not full is its own.
 __device__ __forceinline__ void forkOne(const Books& b, const PageScratch& s, const Requests& q, ListIndex i) {
   const int32_t first = s.request[i], before = s.before[i];
   const int32_t whole = before / b.pageTokens, need = before % b.pageTokens != 0;
@@ -368,6 +364,10 @@ __device__ __forceinline__ void forkOne(const Books& b, const PageScratch& s, co
     b.lengths[child] = before;
   }
 }
+// 512 forks of 8 pools' 16 KiB pages: 16 children read the same page, so loads stay in the caches (25 us for the call; 39
+// if they do not). Two loads a lane: 25 us, four 27, one 33 (every wave looks its request up).
+// The first tableBlocks workgroups (of the first launch, if the pools take several) write the tables, the others copy the
+// contents of the last pages. Neither reads what the other writes: children were empty, and parents stay as they are.
 __global__ __launch_bounds__(kMoveThreads) void forkKernel(Books b, PageScratch s, Requests q, PoolSet p, uint32_t tableBlocks) {
   if (blockIdx.x < tableBlocks) {
     for (ListIndex i = blockIdx.x; i < (ListIndex)q.n; i += tableBlocks) forkOne(b, s, q, i);

@@ -117,7 +117,7 @@ def test_lookup_from_and_to_addresses_aligned_to_an_element_only(dtype):
 
 
 def test_lookup_with_several_rows_a_wave():
-    # from 32768 pieces of 512 elements on a wave takes four tokens' rows; 4099 tokens leave the last one three
+    # from 16384 pieces of 512 elements on a wave takes two tokens' rows; 4099 tokens leave the last one a single one
     t, ids = _randn(12, 9, 4100, dtype=torch.bfloat16), _ids(13, 4099, -1, 10)
     iu.check(_lookup(t, ids, torch.bfloat16, scale=0.7), *iu.lookup(t, ids, 0, 0.7))
 
