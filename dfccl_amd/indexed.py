@@ -12,6 +12,7 @@ import torch
 from . import _lib, api
 
 _FLOATS = frozenset((torch.float32, torch.float16, torch.bfloat16))
+_INT32, _INT64 = (1 << 31) - 1, -(1 << 63)  # the largest, the smallest of the C types
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the current stream's handle without an object
 
 
@@ -98,7 +99,8 @@ def embedding_lookup(table, ids, out, scale=1.0, first_row=0, stream=None):
     if tuple(out.shape) != (tokens, width):
         raise ValueError(f"out has shape {tuple(out.shape)}, not {(tokens, width)}")
     _on(device, out)
-    _fits(64, "first_row", first_row)
+    if not _INT64 <= first_row < -_INT64:
+        _fits(64, "first_row", first_row)
     _call(device, _lib.load().dfcclEmbeddingLookup, "dfcclEmbeddingLookup", table_ptr, api.DTYPE_OF[table.dtype], rows,
           table_stride, first_row, _ids_ptr(ids, device), api.DTYPE_OF[ids.dtype], tokens, width, scale, out_ptr,
           api.DTYPE_OF[out.dtype], out_stride, _stream_of(device, stream))
@@ -241,7 +243,8 @@ class PageCache:
     def _lists(self, *lists):
         """Addresses of the lists, and their common length."""
         n = lists[0].numel()
-        _fits(32, "a list's length", n)
+        if n > _INT32:
+            _fits(32, "a list's length", n)
         for t in lists:
             if t.dtype is not torch.int32:
                 raise TypeError("lists of sequences, pages and lengths are int32 tensors")
