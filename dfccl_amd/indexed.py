@@ -176,8 +176,8 @@ class PageCache:
     bookkeeping, int32 tensors that the caller owns (PageCache.empty makes those of an empty cache).  report[0]:
     requests refused by the last extend or fork; report[1], report[2]: pages moved, pages live at the last compact.
 
-    The report and a workspace are the cache's own memory, taken on the stream that is current in the constructor; the
-    first call on another stream waits for what the constructor needs of that one.  A graph with captured calls uses
+    The report and a workspace (and what empty() makes) are the cache's own memory, taken on the stream that is current in
+    the constructor; the first call on another stream waits for what the constructor needs of that one.  A graph with captured calls uses
     them too: keep the cache as long as the graph, and capture once the constructor's stream has got that far
     (torch.cuda.graph waits for the device)."""
 
@@ -210,6 +210,7 @@ class PageCache:
             tables.shape[0], tables.shape[1], api._dev_ptr(refcounts), api._dev_ptr(tables), api._dev_ptr(lengths),
             api._dev_ptr(self.report), api._dev_ptr(self._workspace), need.value)
         self._ref = ctypes.byref(self._struct)
+        self._own = [self._workspace, self.report]
         # What comes before this place on the constructor's stream may still use the memory, and clears the report.
         self._made_on, self._joined, self._made = _stream_of(device, None), {}, None
         if device.type == "cuda":
@@ -222,8 +223,10 @@ class PageCache:
         """A cache whose pages are all free."""
         def ints(value, *shape):
             return torch.full(shape, value, dtype=torch.int32, device=pools[0].device)
-        return cls(pools, page_tokens, ints(0, pools[0].shape[0]), ints(-1, sequences, pages_per_sequence),
-                   ints(0, sequences))
+        cache = cls(pools, page_tokens, ints(0, pools[0].shape[0]), ints(-1, sequences, pages_per_sequence),
+                    ints(0, sequences))
+        cache._own += [cache.refcounts, cache.tables, cache.lengths]
+        return cache
 
     def _stream(self, stream):
         """The stream's handle, for calls that use the cache's own memory. Another stream than the constructor's waits for
@@ -232,8 +235,8 @@ class PageCache:
         if handle != self._made_on and handle not in self._joined:
             if stream is None:
                 stream = torch.cuda.current_stream(self._device)
-            self._workspace.record_stream(stream)
-            self.report.record_stream(stream)
+            for t in self._own:
+                t.record_stream(stream)
             if not _capturing(stream):  # (a capture may not wait for an event from before it)
                 if self._made is not None:
                     stream.wait_event(self._made)
@@ -276,7 +279,7 @@ class PageCache:
     def free(self, sequences, stream=None):
         """The sequences become empty and give up their pages."""
         _call(self._device, self._lib.dfcclPagesFree, "dfcclPagesFree", self._ref, *self._lists(sequences),
-              _stream_of(self._device, stream))
+              self._stream(stream))
 
     def compact(self, stream=None):
         """Moves pages until the live ones have the lowest numbers; counts and tables follow."""

@@ -148,11 +148,23 @@ def test_a_page_caches_own_memory_is_shared_with_the_streams_that_it_is_used_on(
     assert made_on.waited == [] and cache.report.recorded == [other, third]
 
 
-def test_copy_and_free_use_none_of_it_and_wait_for_nothing(gpu):
+def test_the_bookkeeping_that_empty_makes_is_the_caches_own_memory(gpu, monkeypatch):
+    monkeypatch.setattr(torch, "full", lambda shape, *a, **kw: Buffer(gpu, *shape))
+    other, one = Stream(2, "cuda:0"), Buffer(gpu, 1)
+    cache = dfccl_amd.PageCache.empty([Buffer(gpu, 6, 8)], 4, 3, 2)
+    cache.free(one, stream=other)
+    assert other.waited == ["behind what the constructor needs"]
+    own = (cache.refcounts, cache.tables, cache.lengths, cache.report, cache._workspace)
+    assert [b.recorded for b in own] == [[other]] * 5
+    passed = _cache(gpu)  # (the caller's bookkeeping is the caller's to keep)
+    passed.free(one, stream=other)
+    assert [b.recorded for b in (passed.refcounts, passed.tables, passed.lengths)] == [[]] * 3
+
+
+def test_a_copy_uses_none_of_it_and_waits_for_nothing(gpu):
     cache, other, one = _cache(gpu), Stream(2, "cuda:0"), Buffer(gpu, 1)
     cache.copy(one, one, stream=other)
-    cache.free(one, stream=other)
-    assert [args[-1] for _, args in gpu.calls[-2:]] == [2, 2]
+    assert gpu.calls[-1][1][-1] == 2
     assert other.waited == [] and cache._workspace.recorded == [] and cache.report.recorded == []
 
 

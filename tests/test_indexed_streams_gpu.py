@@ -124,3 +124,22 @@ def test_a_page_cache_captured_first_and_used_on_other_streams_afterwards():
         live = 4096 + 2 * (turn + 1)
         assert cache.lengths.tolist() == [16384, 8 * (turn + 1), 0] and int(cache.report[2]) == live
         assert bool((cache.refcounts[:live] == 1).all()) and not bool(cache.refcounts[live:].any())
+
+
+def test_a_dropped_cache_of_emptys_making_keeps_its_bookkeeping_while_a_call_uses_it():
+    import dfccl_amd
+    s, pools = torch.cuda.Stream(), [torch.zeros(3000, 64, dtype=torch.uint8, device="cuda:0")]
+    warm = dfccl_amd.PageCache.empty(pools, 4, 300, 700)
+    one, many = _ints(0), _ints(*range(300))
+    warm.extend(one, one, stream=s)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        behind = _busy()
+    cache = dfccl_amd.PageCache.empty(pools, 4, 300, 700)
+    sizes = [(t.numel(), t.data_ptr()) for t in (cache.refcounts, cache.tables, cache.lengths)]
+    cache.free(many, stream=s)
+    del cache
+    others = [torch.empty(n, dtype=torch.int32, device="cuda:0") for n, _ in sizes for _ in range(4)]
+    if not behind.query():
+        assert not {at for _, at in sizes} & {o.data_ptr() for o in others}
+    torch.cuda.synchronize()
